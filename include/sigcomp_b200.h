@@ -13,7 +13,9 @@
  *     host memory (pageable or pinned) and do the copies; "_device" entry points
  *     take device pointers already resident on the model's GPU.
  *   - `stream` is a cudaStream_t passed as void*; NULL selects the default stream.
- *     Every entry point returns after its work on `stream` has completed.
+ *     Every entry point returns after its work on `stream` has completed, except the
+ *     int8 operators (sc_quantize_tokens_device and those after it), which return once
+ *     their work is in `stream` and can be captured into a graph.
  *   - Return value: SC_OK or an SC_ERR_* code; sc_last_error() gives the message
  *     (thread-local, valid until the next call on the same thread).
  *   - A chunk is at most `chunk_len` tokens (uint8, the SigComp "small" symbols).
@@ -279,6 +281,62 @@ SC_API int sc_selftest_wait_timeout(sc_model *model, void *stream);
 #define SC_NOALLOC_MAX_WIDTH 512
 SC_API int sc_mlp_logits_device_noalloc(sc_model *model, const int16_t *windows, int64_t rows,
                                         int8_t *logits, void *stream);
+
+/*
+ * int8 operators with a scale for each token (row) and each channel (weight row), for
+ * entropy models that one multiplier per layer does not serve (sc_linear_layer_device has
+ * per-layer scales, as the reference does; these have no counterpart in it).  Results depend
+ * neither on the other rows of a call nor on their number: what an encoder computes in
+ * batches, a decoder computes token by token, bit for bit.
+ *
+ * They take no model: `device` says where the arrays are, and every array is in its memory.
+ * Rows are `stride` elements apart, which may be more than their length; scales and biases
+ * are contiguous.  No state is kept between calls and none is shared, so calls may overlap
+ * on the GPU, given arrays and workspaces of their own.  Types are SC_TYPE_*.
+ * rows 0 is a call that does nothing.
+ *
+ * sc_quantize_tokens_device: for each row, with fl() a rounding to float,
+ *   a = max(max |x|, 2^-100), scale = fl(a / 127), q = rint(x * fl(127 / a)),
+ * the product exact and ties to even.  A row with an infinity or a NaN gets the scale NaN
+ * and zeros.  Bytes between a row's end and the next row's start are left as they are.
+ */
+#define SC_TYPE_F32  0
+#define SC_TYPE_F16  1
+#define SC_TYPE_BF16 2
+#define SC_TYPE_I8   3
+SC_API int sc_quantize_tokens_device(int device, const void *x, int32_t x_type, int64_t rows, int64_t cols,
+                                     int64_t x_stride, int8_t *q, int64_t q_stride, float *scales, void *stream);
+
+/* The values that int8 rows stand for: q * scales[row] in float, rounded once to y's type.
+ * With scales NULL, every row has the scale `scale`. */
+SC_API int sc_dequantize_tokens_device(int device, const int8_t *q, int64_t q_stride, const float *scales,
+                                       float scale, int64_t rows, int64_t cols, void *y, int32_t y_type,
+                                       int64_t y_stride, void *stream);
+
+/*
+ * y[rows][n] = relu(x[rows][k] * w[n][k]^T) with scales and bias, in float:
+ *   fma(fl(fl(sum_k x w) * x_scales[row]), w_scales[channel], bias[channel])
+ * the sum exact (1 <= k <= SC_INT8_MAX_K), relu if nonzero (a NaN stays), bias NULL for none.
+ *   x   int8 with x_scales [rows], or SC_TYPE_F32 / F16 / BF16 (x_scales NULL): quantised
+ *       first, as by sc_quantize_tokens_device
+ *   y   SC_TYPE_F32 / F16 / BF16: rounded once to the type; or SC_TYPE_I8: with y_scales
+ *       [rows] (output) quantised as by sc_quantize_tokens_device, with y_scales NULL as
+ *       rint(fl(y / output_scale)), saturated (the int8 logits of sc_encode_logits_device;
+ *       a NaN becomes 0)
+ *   workspace   device memory, 256-byte aligned, of at least the bytes that
+ *               sc_int8_linear_workspace gives for the same arguments; NULL if that is 0
+ * y, y_scales and workspace overlap no input.
+ */
+#define SC_INT8_MAX_K 131071
+SC_API int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_stride, const float *x_scales,
+                                 const int8_t *w, int64_t w_stride, const float *w_scales, const float *bias,
+                                 int64_t rows, int64_t n, int64_t k, int32_t relu, void *y, int32_t y_type,
+                                 int64_t y_stride, float *y_scales, float output_scale, void *workspace,
+                                 int64_t workspace_bytes, void *stream);
+
+/* Workspace of a call with these arguments, whatever its addresses (host only). */
+SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int64_t x_stride, int64_t w_stride, int64_t rows, int64_t n,
+                                        int64_t k, int32_t y_type);
 
 /*
  * Per-launch CUDA-event timing (no counterpart in the reference; instrumentation

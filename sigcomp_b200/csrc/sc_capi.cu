@@ -1,12 +1,14 @@
 // extern "C" boundary of libsigcomp_b200 (declared in include/sigcomp_b200.h).
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cstdarg>
 #include <cstring>
 #include <memory>
 #include <new>
 
 #include "../../include/sigcomp_b200.h"
+#include "sc_int8.h"
 #include "sc_internal.h"
 
 namespace sc {
@@ -68,12 +70,29 @@ int map_cuda(const CudaError &e)
     return e.code == cudaErrorMemoryAllocation ? SC_ERR_OUT_OF_MEMORY : SC_ERR_CUDA;
 }
 
+// Runs f with `device` current and turns every exception into a status.
+template <typename F>
+int guarded_on(int device, F &&f)
+{
+    try {
+        DeviceGuard g(device);
+        SC_CUDA(g.err);
+        return f();
+    } catch (const CudaError &e) {
+        return map_cuda(e);
+    } catch (const std::bad_alloc &) {
+        set_error("host out of memory");
+        return SC_ERR_OUT_OF_MEMORY;
+    } catch (...) {
+        set_error("internal error");
+        return SC_ERR_CUDA;
+    }
+}
+
 template <typename F>
 int guarded(sc_model *m, F &&f)
 {
-    try {
-        DeviceGuard g(m->device);
-        SC_CUDA(g.err);
+    return guarded_on(m->device, [&]() -> int {
         int rc = f();
         if (m->prof.on) {
             SC_CUDA(cudaDeviceSynchronize());
@@ -84,15 +103,7 @@ int guarded(sc_model *m, F &&f)
             return SC_ERR_CUDA;
         }
         return rc;
-    } catch (const CudaError &e) {
-        return map_cuda(e);
-    } catch (const std::bad_alloc &) {
-        set_error("host out of memory");
-        return SC_ERR_OUT_OF_MEMORY;
-    } catch (...) {
-        set_error("internal error");
-        return SC_ERR_CUDA;
-    }
+    });
 }
 
 // validate chunk offsets on the host; returns SC_OK or sets the error
@@ -130,6 +141,12 @@ int check_auto_path(const sc_model *m, bool fused)
         return SC_ERR_UNSUPPORTED;
     }
     return SC_OK;
+}
+
+// rows of `cols` elements that the kernels' index types reach, at least `cols` apart
+bool rows_ok(int64_t rows, int64_t cols, int64_t stride)
+{
+    return rows >= 0 && rows < (1ll << 31) - 1024 && cols >= 1 && cols <= (1ll << 30) && stride >= cols;
 }
 
 int first_error(const uint8_t *errs, int64_t n)
@@ -743,6 +760,82 @@ int sc_linear_layer_device(sc_model *m, int32_t layer, const int8_t *x, int64_t 
     return guarded(m, [&]() -> int {
         linear_tc(m, layer, x, rows, y, s);
         SC_CUDA(cudaStreamSynchronize(s));
+        return SC_OK;
+    });
+}
+
+int sc_quantize_tokens_device(int device, const void *x, int32_t x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                              int8_t *q, int64_t q_stride, float *scales, void *stream)
+{
+    g_err[0] = 0;
+    if (x_type < SC_TYPE_F32 || x_type > SC_TYPE_BF16 || !rows_ok(rows, cols, q_stride) || x_stride < 0 ||
+        (rows > 0 && (!x || !q || !scales))) {
+        set_error("invalid argument");
+        return SC_ERR_INVALID_ARGUMENT;
+    }
+    if (rows == 0) return SC_OK;
+    return guarded_on(device, [&]() -> int {
+        quantize_tokens(x, x_type, rows, cols, x_stride, q, q_stride, scales, (cudaStream_t)stream);
+        return SC_OK;
+    });
+}
+
+int sc_dequantize_tokens_device(int device, const int8_t *q, int64_t q_stride, const float *scales, float scale,
+                                int64_t rows, int64_t cols, void *y, int32_t y_type, int64_t y_stride, void *stream)
+{
+    g_err[0] = 0;
+    if (y_type < SC_TYPE_F32 || y_type > SC_TYPE_BF16 || !rows_ok(rows, cols, y_stride) || q_stride < 0 ||
+        (rows > 0 && (!q || !y))) {
+        set_error("invalid argument");
+        return SC_ERR_INVALID_ARGUMENT;
+    }
+    if (rows == 0) return SC_OK;
+    return guarded_on(device, [&]() -> int {
+        dequantize_tokens(q, q_stride, scales, scale, rows, cols, y, y_type, y_stride, (cudaStream_t)stream);
+        return SC_OK;
+    });
+}
+
+int64_t sc_int8_linear_workspace(int32_t x_type, int64_t x_stride, int64_t w_stride, int64_t rows, int64_t n, int64_t k,
+                                 int32_t y_type)
+{
+    Int8Linear p{};
+    p.x_type = x_type;
+    p.x_stride = x_stride;
+    p.w_stride = w_stride;
+    p.rows = rows;
+    p.n = n;
+    p.k = k;
+    p.y_type = y_type;
+    return rows > 0 ? int8_linear_workspace(p) : 0;
+}
+
+int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_stride, const float *x_scales,
+                          const int8_t *w, int64_t w_stride, const float *w_scales, const float *bias, int64_t rows,
+                          int64_t n, int64_t k, int32_t relu, void *y, int32_t y_type, int64_t y_stride,
+                          float *y_scales, float output_scale, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    g_err[0] = 0;
+    if (x_type < SC_TYPE_F32 || x_type > SC_TYPE_I8 || y_type < SC_TYPE_F32 || y_type > SC_TYPE_I8 ||
+        k > SC_INT8_MAX_K || !rows_ok(rows, n, y_stride) || !rows_ok(n, k, w_stride) || x_stride < 0 || !w ||
+        !w_scales || (rows > 0 && (!x || !y)) || (rows > 0 && (x_type == SC_TYPE_I8) != (x_scales != nullptr))) {
+        set_error("invalid argument");
+        return SC_ERR_INVALID_ARGUMENT;
+    }
+    if (rows == 0) return SC_OK;
+    if (y_type == SC_TYPE_I8 && !y_scales && !(output_scale > 0 && output_scale <= FLT_MAX)) {
+        set_error("output_scale must be a finite positive number");
+        return SC_ERR_INVALID_ARGUMENT;
+    }
+    Int8Linear p{x, x_type, x_stride, x_scales, w,        w_stride, w_scales,     bias,     rows, n,
+                 k, relu,   y,        y_type,   y_stride, y_scales, output_scale, workspace};
+    const int64_t need = int8_linear_workspace(p);
+    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) != 0)) {
+        set_error("workspace of %lld bytes, 256-byte aligned, needed", (long long)need);
+        return SC_ERR_INVALID_ARGUMENT;
+    }
+    return guarded_on(device, [&]() -> int {
+        int8_linear(p, (cudaStream_t)stream);
         return SC_OK;
     });
 }

@@ -1,0 +1,371 @@
+// int8 operators with a scale for each token and channel.
+//
+//   quantise     a = max(max_k |x_k|, 2^-100), s = fl(a / 127), r = fl(127 / a), q = rint(x r)
+//   product      y_ij = relu(fma(fl(fl(sum_k q_ik w_jk) s_i), t_j, b_j)), rounded to its type
+//   requantise   the product's rows in 32 bits, quantised as above or by one given scale
+//
+// Sums of products are whole numbers below 2^31 (k <= 131,071) and exact in int32, so a result
+// does not depend on the kernel, the tile or the split of K that computed it; the roundings
+// after the sum are fixed above.  A decoder that works token by token therefore reproduces what
+// an encoder computed in batches.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "sc_internal.h"
+#include "sc_int8.h"
+
+namespace sc {
+namespace {
+
+// ---- element types ---------------------------------------------------------------------------
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// ---- a row's scale ---------------------------------------------------------------------------
+// Magnitudes are compared as bit patterns: for floats without their sign the order of the bits is
+// the order of the values, infinity and NaN above all others, so one whole-number maximum also
+// tells whether the row holds a value that cannot be quantised.
+constexpr uint32_t kInfBits = 0x7f800000u;
+constexpr uint32_t kSmallestBits = 0x0d800000u;      // 2^-100: 127 / a stays finite
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+struct RowScale {
+    float s, r;          // scale and reciprocal; both zero when the row cannot be quantised
+    bool finite;
+};
+
+__device__ __forceinline__ RowScale row_scale(uint32_t top)
+{
+    RowScale o;
+    o.finite = top < kInfBits;
+    const float a = __uint_as_float(max(top, kSmallestBits));
+    o.s = __fdiv_rn(a, 127.0f);
+    o.r = __fdiv_rn(127.0f, a);
+    return o;
+}
+
+// rint(v r) in the low byte.  The sum with 1.5 * 2^23 has a unit in the last place of one, so the
+// fused multiply-add rounds the exact product to a whole number, ties to even, in one rounding.
+// |v r| <= 127 (1 + 2^-24), so nothing saturates.
+__device__ __forceinline__ uint32_t quantise_bits(float v, float r) { return __float_as_uint(__fmaf_rn(v, r, 12582912.0f)); }
+
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// ---- quantise --------------------------------------------------------------------------------
+// A row is read once: T threads hold its 16-byte vectors in registers through the maximum.
+// Bound by HBM (e + 1 bytes per element).
+template <typename T, int THREADS, int HELD, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
+k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ q, int64_t q_stride,
+           float *__restrict__ scales)
+{
+    constexpr int V = 16 / sizeof(T);
+    constexpr int PER_BLOCK = THREADS < 256 ? 256 / THREADS : 1;
+    __shared__ uint32_t tops[32];
+    const int t = threadIdx.x % THREADS;
+    const int64_t row = (int64_t)blockIdx.x * PER_BLOCK + threadIdx.x / THREADS;
+    if (THREADS <= 32 && row >= rows) return;        // whole warps: THREADS divides 32's multiples
+    const T *xr = x + row * x_stride;
+    float v[HELD][V];
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int c = (h * THREADS + t) * V;
+        if (ALIGNED && c + V <= cols) {
+            const uint4 raw = *reinterpret_cast<const uint4 *>(xr + c);
+            const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[h][i] = to_f32<T>(e[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[h][i] = c + i < cols ? to_f32<T>(xr[c + i]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = max(top, magnitude(v[h][i]));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (THREADS > 32) {
+        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+        __syncthreads();
+        const int w = threadIdx.x & 31;
+        top = __reduce_max_sync(0xffffffffu, w < THREADS / 32 ? tops[w] : 0u);
+    }
+    const RowScale rs = row_scale(top);
+    if (t == 0) scales[row] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+    int8_t *qr = q + row * q_stride;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int c = (h * THREADS + t) * V;
+        uint32_t p[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i)
+            p[i] = rs.finite ? pack4(quantise_bits(v[h][4 * i], rs.r), quantise_bits(v[h][4 * i + 1], rs.r),
+                                     quantise_bits(v[h][4 * i + 2], rs.r), quantise_bits(v[h][4 * i + 3], rs.r))
+                             : 0u;
+        if (ALIGNED && c + V <= cols) {
+            if (V == 8) *reinterpret_cast<uint2 *>(qr + c) = make_uint2(p[0], p[V / 4 - 1]);
+            else *reinterpret_cast<uint32_t *>(qr + c) = p[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (c + i < cols) qr[c + i] = (int8_t)(p[i / 4] >> (8 * (i % 4)));
+        }
+    }
+}
+
+// Rows longer than a block holds: read twice, the second time mostly from L2.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__restrict__ q, int64_t q_stride,
+                float *__restrict__ scales)
+{
+    __shared__ uint32_t tops[32];
+    const T *xr = x + (int64_t)blockIdx.x * x_stride;
+    uint32_t top = 0;
+    for (int c = threadIdx.x; c < cols; c += 1024) top = max(top, magnitude(to_f32<T>(xr[c])));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, tops[threadIdx.x & 31]);
+    const RowScale rs = row_scale(top);
+    if (threadIdx.x == 0) scales[blockIdx.x] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+    int8_t *qr = q + (int64_t)blockIdx.x * q_stride;
+    for (int c = threadIdx.x; c < cols; c += 1024)
+        qr[c] = rs.finite ? (int8_t)quantise_bits(to_f32<T>(xr[c]), rs.r) : 0;
+}
+
+// ---- dequantise ------------------------------------------------------------------------------
+// One warp per 512 columns of a row, 16 values a thread.  Bound by HBM (1 + e bytes per element).
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256)
+k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__restrict__ scales, float scale, int64_t rows,
+             int cols, T *__restrict__ y, int64_t y_stride)
+{
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const float s = scales ? scales[row] : scale;
+    const int8_t *qr = q + row * q_stride;
+    T *yr = y + row * y_stride;
+    for (int64_t c0 = (int64_t)blockIdx.y * 512; c0 < cols; c0 += (int64_t)gridDim.y * 512) {
+        const int c = (int)c0 + (threadIdx.x & 31) * 16;
+        if (ALIGNED && c + 16 <= cols) {
+            const uint4 raw = *reinterpret_cast<const uint4 *>(qr + c);
+            const int8_t *e = reinterpret_cast<const int8_t *>(&raw);
+            __align__(16) T out[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) out[i] = from_f32<T>(__fmul_rn((float)e[i], s));
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T); ++i)
+                reinterpret_cast<uint4 *>(yr + c)[i] = reinterpret_cast<const uint4 *>(out)[i];
+        } else {
+            for (int i = 0; i < 16 && c + i < cols; ++i) yr[c + i] = from_f32<T>(__fmul_rn((float)qr[c + i], s));
+        }
+    }
+}
+
+// ---- product ---------------------------------------------------------------------------------
+// Roundings of one result, see the head of this file.  max.NaN keeps a NaN that the scale carries.
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+__device__ __forceinline__ float affine(int32_t acc, float s, float t, float b, int relu)
+{
+    const float y = __fmaf_rn(__fmul_rn(__int2float_rn(acc), s), t, b);
+    return relu ? max_nan(y, 0.0f) : y;
+}
+
+// Any sizes, strides and alignment: 64 x 64 results a block, K in blocks of 64, CUDA cores.
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_product_any(const int8_t *__restrict__ x, int64_t x_stride, const float *__restrict__ xs, const int8_t *__restrict__ w,
+              int64_t w_stride, const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int n, int k,
+              int relu, T *__restrict__ y, int64_t y_stride)
+{
+    __shared__ int32_t a[64][17], b[64][17];
+    const int64_t m0 = (int64_t)blockIdx.x * 64;
+    const int n0 = blockIdx.y * 64;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    int32_t acc[4][4] = {};
+    for (int k0 = 0; k0 < k; k0 += 64) {
+        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+            const int r = i >> 6, c = i & 63;
+            const bool in = k0 + c < k;
+            reinterpret_cast<int8_t *>(a[r])[c] = in && m0 + r < rows ? x[(m0 + r) * x_stride + k0 + c] : 0;
+            reinterpret_cast<int8_t *>(b[r])[c] = in && n0 + r < n ? w[(int64_t)(n0 + r) * w_stride + k0 + c] : 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[ty + 16 * i][c], b[tx + 16 * j][c], acc[i][j]);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = m0 + ty + 16 * i;
+            const int c = n0 + tx + 16 * j;
+            if (r < rows && c < n)
+                y[r * y_stride + c] = from_f32<T>(affine(acc[i][j], xs[r], ws[c], bias ? bias[c] : 0.0f, relu));
+        }
+}
+
+// Rows in 32 bits to int8 by one given scale: sat(rint(y / scale)); a NaN becomes 0.
+__global__ void __launch_bounds__(256)
+k_static(const float *__restrict__ y, int64_t rows, int cols, float scale, int8_t *__restrict__ q, int64_t q_stride)
+{
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    for (int c = threadIdx.x & 31; c < cols; c += 32) {
+        int32_t o;
+        asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(o) : "f"(__fdiv_rn(y[row * cols + c], scale)));
+        q[row * q_stride + c] = (int8_t)o;
+    }
+}
+
+bool aligned(const void *p, int64_t stride_bytes, int a)
+{
+    return ((uintptr_t)p % a) == 0 && stride_bytes % a == 0;
+}
+
+unsigned grid_x(int64_t blocks)
+{
+    if (blocks > INT_MAX) throw CudaError{cudaErrorInvalidValue, "too many rows for one launch"};
+    return (unsigned)blocks;
+}
+
+template <typename T>
+void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t qs, float *scales, cudaStream_t s)
+{
+    constexpr int V = 16 / sizeof(T);
+    const bool al = aligned(x, xs * (int64_t)sizeof(T), 16) && aligned(q, qs, V);
+#define SC_Q(THREADS, HELD)                                                                                        \
+    do {                                                                                                           \
+        const unsigned g = grid_x(THREADS < 256 ? (rows + 256 / THREADS - 1) / (256 / THREADS) : rows);            \
+        if (al) k_quantize<T, THREADS, HELD, true><<<g, THREADS < 256 ? 256 : THREADS, 0, s>>>(x, rows, cols, xs, q, qs, scales); \
+        else k_quantize<T, THREADS, HELD, false><<<g, THREADS < 256 ? 256 : THREADS, 0, s>>>(x, rows, cols, xs, q, qs, scales);   \
+    } while (0)
+    if (cols <= 32 * V) SC_Q(32, 1);
+    else if (cols <= 64 * V) SC_Q(32, 2);
+    else if (cols <= 128 * V) SC_Q(32, 4);
+    else if (cols <= 256 * V) SC_Q(256, 1);
+    else if (cols <= 512 * V) SC_Q(256, 2);
+    else if (cols <= 1024 * V) SC_Q(1024, 1);
+    else if (cols <= 4096 * V) SC_Q(1024, 4);
+    else k_quantize_long<T><<<grid_x(rows), 1024, 0, s>>>(x, cols, xs, q, qs, scales);
+#undef SC_Q
+    SC_LAUNCH_CHECK();
+    count_launch();
+}
+
+template <typename T>
+void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, int64_t rows, int cols, T *y, int64_t ys,
+                cudaStream_t s)
+{
+    const dim3 g(grid_x((rows + 7) / 8), (unsigned)std::min((cols + 511) / 512, 65535));
+    if (aligned(q, qs, 16) && aligned(y, ys * (int64_t)sizeof(T), 16))
+        k_dequantize<T, true><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys);
+    else
+        k_dequantize<T, false><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys);
+    SC_LAUNCH_CHECK();
+    count_launch();
+}
+
+template <typename T>
+void product(const Int8Linear &p, const int8_t *x, int64_t x_stride, const float *xs, T *y, int64_t y_stride,
+             cudaStream_t s)
+{
+    const dim3 g(grid_x((p.rows + 63) / 64), (unsigned)((p.n + 63) / 64));
+    k_product_any<T><<<g, 256, 0, s>>>(x, x_stride, xs, p.w, p.w_stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k,
+                                       p.relu, y, y_stride);
+    SC_LAUNCH_CHECK();
+    count_launch();
+}
+
+int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+}  // namespace
+
+void quantize_tokens(const void *x, int type, int64_t rows, int64_t cols, int64_t x_stride, int8_t *q, int64_t q_stride,
+                     float *scales, cudaStream_t s)
+{
+    if (type == SC_TYPE_F32) quantize((const float *)x, rows, (int)cols, x_stride, q, q_stride, scales, s);
+    else if (type == SC_TYPE_F16) quantize((const __half *)x, rows, (int)cols, x_stride, q, q_stride, scales, s);
+    else quantize((const __nv_bfloat16 *)x, rows, (int)cols, x_stride, q, q_stride, scales, s);
+}
+
+void dequantize_tokens(const int8_t *q, int64_t q_stride, const float *scales, float scale, int64_t rows, int64_t cols,
+                       void *y, int type, int64_t y_stride, cudaStream_t s)
+{
+    if (type == SC_TYPE_F32) dequantize(q, q_stride, scales, scale, rows, (int)cols, (float *)y, y_stride, s);
+    else if (type == SC_TYPE_F16) dequantize(q, q_stride, scales, scale, rows, (int)cols, (__half *)y, y_stride, s);
+    else dequantize(q, q_stride, scales, scale, rows, (int)cols, (__nv_bfloat16 *)y, y_stride, s);
+}
+
+// Workspace: the rows of a float x held in 8 bits and their scales, then the product's rows in 32
+// bits where they come back quantised.
+int64_t int8_linear_workspace(const Int8Linear &p)
+{
+    int64_t b = 0;
+    if (p.x_type != SC_TYPE_I8) b += pad(p.rows * pad(p.k, 16), 256) + pad(p.rows * 4, 256);
+    if (p.y_type == SC_TYPE_I8) b += pad(p.rows * p.n * 4, 256);
+    return b;
+}
+
+void int8_linear(const Int8Linear &p, cudaStream_t s)
+{
+    uint8_t *ws = (uint8_t *)p.workspace;
+    const int8_t *x = (const int8_t *)p.x;
+    int64_t x_stride = p.x_stride;
+    const float *xs = p.x_scales;
+    if (p.x_type != SC_TYPE_I8) {
+        int8_t *q = (int8_t *)ws;
+        x_stride = pad(p.k, 16);
+        ws += pad(p.rows * x_stride, 256);
+        float *sc = (float *)ws;
+        ws += pad(p.rows * 4, 256);
+        quantize_tokens(p.x, p.x_type, p.rows, p.k, p.x_stride, q, x_stride, sc, s);
+        x = q;
+        xs = sc;
+    }
+    if (p.y_type == SC_TYPE_F32) product(p, x, x_stride, xs, (float *)p.y, p.y_stride, s);
+    else if (p.y_type == SC_TYPE_F16) product(p, x, x_stride, xs, (__half *)p.y, p.y_stride, s);
+    else if (p.y_type == SC_TYPE_BF16) product(p, x, x_stride, xs, (__nv_bfloat16 *)p.y, p.y_stride, s);
+    else {
+        float *y = (float *)ws;
+        product(p, x, x_stride, xs, y, p.n, s);
+        if (p.y_scales) {
+            quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+        } else {
+            k_static<<<grid_x((p.rows + 7) / 8), 256, 0, s>>>(y, p.rows, (int)p.n, p.output_scale, (int8_t *)p.y, p.y_stride);
+            SC_LAUNCH_CHECK();
+            count_launch();
+        }
+    }
+}
+
+}  // namespace sc
