@@ -334,9 +334,16 @@ SC_API int sc_int8_linear_device(int device, const void *x, int32_t x_type, int6
                                  int64_t y_stride, float *y_scales, float output_scale, void *workspace,
                                  int64_t workspace_bytes, void *stream);
 
-/* Workspace of a call with these arguments, whatever its addresses (host only). */
-SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int64_t x_stride, int64_t w_stride, int64_t rows, int64_t n,
-                                        int64_t k, int32_t y_type);
+/* Workspace of a call with these arguments (host only).  x_packed (for an int8 x) and w_packed:
+ * nonzero when the address and the stride are multiples of 16 and rows do not overlap; arrays
+ * that are not are copied into the workspace first.  y_scaled: nonzero when y_scales is given. */
+SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_packed, int64_t rows, int64_t n,
+                                        int64_t k, int32_t y_type, int32_t y_scaled);
+
+/* Waits for `stream` and reports whether a device-side wait of an int8 operator has timed out on
+ * the device since the last such report (SC_ERR_CUDA, as the other entry points report it; the
+ * results of the calls since then are not to be used). */
+SC_API int sc_int8_status_device(int device, void *stream);
 
 /*
  * Per-launch CUDA-event timing (no counterpart in the reference; instrumentation

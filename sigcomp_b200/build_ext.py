@@ -20,8 +20,8 @@ FLAGS = [
 # Kernels whose tcgen05.ld results land in registers asynchronously (until tcgen05.wait::ld):
 # a register spill placed between a load and its wait would store values not yet written, so the
 # build refuses any spill in them.  ptxas -v reports stack and spills per entry function.
-NO_SPILL_KERNELS = ("k_fused2", "k_small_decode")
-NO_SPILL_SOURCE = "sc_mlp_tc.cu"
+NO_SPILL_KERNELS = ("k_fused2", "k_small_decode", "k_pair")
+NO_SPILL_SOURCES = ("sc_mlp_tc.cu", "sc_int8.cu")
 
 
 def spilling_kernels(ptxas_log, names=NO_SPILL_KERNELS):
@@ -59,7 +59,7 @@ def build(force=False, verbose=False, jobs=4):
     procs = []
     for src in SOURCES:
         obj = build_dir / (src + ".o")
-        extra = ["-Xptxas", "-v"] if src == NO_SPILL_SOURCE else []
+        extra = ["-Xptxas", "-v"] if src in NO_SPILL_SOURCES else []
         cmd = [NVCC, *FLAGS, *extra, "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd))
@@ -71,7 +71,7 @@ def build(force=False, verbose=False, jobs=4):
         if p.returncode != 0:
             failed.append((src, out.decode()))
             continue
-        if src == NO_SPILL_SOURCE:
+        if src in NO_SPILL_SOURCES:
             spills = spilling_kernels(out.decode())
             if spills:
                 failed.append((src, "register spills in kernels that must not spill: " + "; ".join(

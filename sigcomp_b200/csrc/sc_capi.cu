@@ -796,17 +796,19 @@ int sc_dequantize_tokens_device(int device, const int8_t *q, int64_t q_stride, c
     });
 }
 
-int64_t sc_int8_linear_workspace(int32_t x_type, int64_t x_stride, int64_t w_stride, int64_t rows, int64_t n, int64_t k,
-                                 int32_t y_type)
+int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_packed, int64_t rows, int64_t n, int64_t k,
+                                 int32_t y_type, int32_t y_scaled)
 {
     Int8Linear p{};
+    float some = 0;
     p.x_type = x_type;
-    p.x_stride = x_stride;
-    p.w_stride = w_stride;
+    p.x_packed = x_packed;
+    p.w_packed = w_packed;
     p.rows = rows;
     p.n = n;
     p.k = k;
     p.y_type = y_type;
+    p.y_scales = y_scaled ? &some : nullptr;
     return rows > 0 ? int8_linear_workspace(p) : 0;
 }
 
@@ -829,6 +831,9 @@ int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_s
     }
     Int8Linear p{x, x_type, x_stride, x_scales, w,        w_stride, w_scales,     bias,     rows, n,
                  k, relu,   y,        y_type,   y_stride, y_scales, output_scale, workspace};
+    // rows at least their length apart: a repeated row (stride 0) is spread
+    p.x_packed = ((uintptr_t)x & 15) == 0 && (x_stride & 15) == 0 && x_stride >= k;
+    p.w_packed = ((uintptr_t)w & 15) == 0 && (w_stride & 15) == 0;
     const int64_t need = int8_linear_workspace(p);
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) != 0)) {
         set_error("workspace of %lld bytes, 256-byte aligned, needed", (long long)need);
@@ -836,6 +841,19 @@ int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_s
     }
     return guarded_on(device, [&]() -> int {
         int8_linear(p, (cudaStream_t)stream);
+        return SC_OK;
+    });
+}
+
+int sc_int8_status_device(int device, void *stream)
+{
+    g_err[0] = 0;
+    return guarded_on(device, [&]() -> int {
+        SC_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+        if (int8_device_error()) {
+            set_error("a device-side wait timed out (kernel gave up after its time limit)");
+            return SC_ERR_CUDA;
+        }
         return SC_OK;
     });
 }

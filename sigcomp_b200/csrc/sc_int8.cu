@@ -13,10 +13,12 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "sc_internal.h"
 #include "sc_int8.h"
+#include "sc_tc.cuh"
 
 namespace sc {
 namespace {
@@ -234,6 +236,16 @@ k_product_any(const int8_t *__restrict__ x, int64_t x_stride, const float *__res
         }
 }
 
+}  // namespace
+}  // namespace sc
+
+#include "sc_int8_mm.cuh"
+
+namespace sc {
+namespace {
+
+// ---- host side -------------------------------------------------------------------------------
+
 // Rows in 32 bits to int8 by one given scale: sat(rint(y / scale)); a NaN becomes 0.
 __global__ void __launch_bounds__(256)
 k_static(const float *__restrict__ y, int64_t rows, int cols, float scale, int8_t *__restrict__ q, int64_t q_stride)
@@ -244,6 +256,23 @@ k_static(const float *__restrict__ y, int64_t rows, int cols, float scale, int8_
         int32_t o;
         asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(o) : "f"(__fdiv_rn(y[row * cols + c], scale)));
         q[row * q_stride + c] = (int8_t)o;
+    }
+}
+
+// Rows copied to a multiple of 16 bytes apart, for arrays that TMA cannot read as they lie.  Bytes behind
+// a row's end stay as they are: the tensor map ends with the row.
+__global__ void __launch_bounds__(256)
+k_spread(const int8_t *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ y, int64_t y_stride)
+{
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    const int8_t *xr = x + row * x_stride;
+    for (int c = (threadIdx.x & 31) * 4; c < cols; c += 128) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < cols) v |= (uint32_t)(uint8_t)xr[c + i] << (8 * i);
+        *reinterpret_cast<uint32_t *>(y + row * y_stride + c) = v;
     }
 }
 
@@ -295,13 +324,67 @@ void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, i
     count_launch();
 }
 
-template <typename T>
-void product(const Int8Linear &p, const int8_t *x, int64_t x_stride, const float *xs, T *y, int64_t y_stride,
-             cudaStream_t s)
+struct Rows8 {
+    const int8_t *p;
+    int64_t stride;
+};
+
+int sm_count()
 {
-    const dim3 g(grid_x((p.rows + 63) / 64), (unsigned)((p.n + 63) / 64));
-    k_product_any<T><<<g, 256, 0, s>>>(x, x_stride, xs, p.w, p.w_stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k,
-                                       p.relu, y, y_stride);
+    static int counts[64];
+    int dev = 0;
+    SC_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && counts[dev] > 0) return counts[dev];
+    int n = 0;
+    SC_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) counts[dev] = n;
+    return n;
+}
+
+// The kernel's shared memory limit, set once per device.
+template <typename F>
+void allow_smem(F *kernel, int bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    SC_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+    SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+template <typename T> constexpr CUtensorMapDataType map_type();
+template <> constexpr CUtensorMapDataType map_type<float>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
+template <> constexpr CUtensorMapDataType map_type<__half>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+template <> constexpr CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+template <> constexpr CUtensorMapDataType map_type<int8_t>() { return CU_TENSOR_MAP_DATA_TYPE_UINT8; }
+
+// y (T; int8: requantised with a scale for each row, at most 512 channels) of int8 rows, on SM pairs
+template <typename T>
+void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, cudaStream_t s)
+{
+    constexpr bool REQUANT = sizeof(T) == 1;
+    static std::atomic<uint64_t> ready{0};
+    allow_smem(k_pair<T, REQUANT>, P_SMEM, ready);
+    PairParams a;
+    a.x = tensor_map(x.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.rows, x.stride, PK, PM);
+    a.w = tensor_map(w.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.n, w.stride, PK, PN / 2);
+    a.y_tma = aligned(y, y_stride * (int64_t)sizeof(T), 16);
+    if (a.y_tma) a.y = tensor_map(y, map_type<T>(), p.n, p.rows, y_stride * sizeof(T), 128 / sizeof(T), 32);
+    a.xs = xs;
+    a.ws = p.w_scales;
+    a.bias = p.bias;
+    a.rows = p.rows;
+    a.n = (int)p.n;
+    a.k = (int)p.k;
+    a.relu = p.relu;
+    a.yp = y;
+    a.y_stride = y_stride;
+    a.y_scales = p.y_scales;
+    const int64_t tiles = (p.rows + 2 * PM - 1) / (2 * PM), units = (p.n + PN - 1) / PN;
+    const int64_t work = REQUANT ? tiles : tiles * units;
+    const unsigned pairs = (unsigned)std::min<int64_t>(work, sm_count() / 2);
+    k_pair<T, REQUANT><<<2 * pairs, P_THREADS, P_SMEM, s>>>(a);
     SC_LAUNCH_CHECK();
     count_launch();
 }
@@ -326,38 +409,54 @@ void dequantize_tokens(const int8_t *q, int64_t q_stride, const float *scales, f
     else dequantize(q, q_stride, scales, scale, rows, (int)cols, (__nv_bfloat16 *)y, y_stride, s);
 }
 
-// Workspace: the rows of a float x held in 8 bits and their scales, then the product's rows in 32
-// bits where they come back quantised.
+// Workspace: the rows of a float x held in 8 bits and their scales, x and w spread where TMA cannot read
+// them, and the product's rows in 32 bits where they come back quantised by a launch of their own.
+static bool own_requant(const Int8Linear &p) { return p.y_type == SC_TYPE_I8 && !(p.y_scales && p.n <= 2 * PN); }
+
 int64_t int8_linear_workspace(const Int8Linear &p)
 {
     int64_t b = 0;
-    if (p.x_type != SC_TYPE_I8) b += pad(p.rows * pad(p.k, 16), 256) + pad(p.rows * 4, 256);
-    if (p.y_type == SC_TYPE_I8) b += pad(p.rows * p.n * 4, 256);
+    if (p.x_type != SC_TYPE_I8) b += pad(p.rows * 4, 256);
+    if (p.x_type != SC_TYPE_I8 || !p.x_packed) b += pad(p.rows * pad(p.k, 16), 256);
+    if (!p.w_packed) b += pad(p.n * pad(p.k, 16), 256);
+    if (own_requant(p)) b += pad(p.rows * p.n * 4, 256);
     return b;
 }
 
 void int8_linear(const Int8Linear &p, cudaStream_t s)
 {
     uint8_t *ws = (uint8_t *)p.workspace;
-    const int8_t *x = (const int8_t *)p.x;
-    int64_t x_stride = p.x_stride;
+    auto take = [&](int64_t bytes) {
+        uint8_t *at = ws;
+        ws += pad(bytes, 256);
+        return at;
+    };
+    auto spread = [&](const int8_t *from, int64_t rows, int64_t stride) {
+        int8_t *to = (int8_t *)take(rows * pad(p.k, 16));
+        k_spread<<<grid_x((rows + 7) / 8), 256, 0, s>>>(from, rows, (int)p.k, stride, to, pad(p.k, 16));
+        SC_LAUNCH_CHECK();
+        count_launch();
+        return Rows8{to, pad(p.k, 16)};
+    };
+    Rows8 x{(const int8_t *)p.x, p.x_stride}, w{p.w, p.w_stride};
     const float *xs = p.x_scales;
     if (p.x_type != SC_TYPE_I8) {
-        int8_t *q = (int8_t *)ws;
-        x_stride = pad(p.k, 16);
-        ws += pad(p.rows * x_stride, 256);
-        float *sc = (float *)ws;
-        ws += pad(p.rows * 4, 256);
-        quantize_tokens(p.x, p.x_type, p.rows, p.k, p.x_stride, q, x_stride, sc, s);
-        x = q;
+        float *sc = (float *)take(p.rows * 4);
+        int8_t *q = (int8_t *)take(p.rows * pad(p.k, 16));
+        quantize_tokens(p.x, p.x_type, p.rows, p.k, p.x_stride, q, pad(p.k, 16), sc, s);
+        x = {q, pad(p.k, 16)};
         xs = sc;
+    } else if (!p.x_packed) {
+        x = spread(x.p, p.rows, x.stride);
     }
-    if (p.y_type == SC_TYPE_F32) product(p, x, x_stride, xs, (float *)p.y, p.y_stride, s);
-    else if (p.y_type == SC_TYPE_F16) product(p, x, x_stride, xs, (__half *)p.y, p.y_stride, s);
-    else if (p.y_type == SC_TYPE_BF16) product(p, x, x_stride, xs, (__nv_bfloat16 *)p.y, p.y_stride, s);
+    if (!p.w_packed) w = spread(p.w, p.n, p.w_stride);
+    if (p.y_type == SC_TYPE_F32) product_pairs(p, x, xs, w, (float *)p.y, p.y_stride, s);
+    else if (p.y_type == SC_TYPE_F16) product_pairs(p, x, xs, w, (__half *)p.y, p.y_stride, s);
+    else if (p.y_type == SC_TYPE_BF16) product_pairs(p, x, xs, w, (__nv_bfloat16 *)p.y, p.y_stride, s);
+    else if (!own_requant(p)) product_pairs(p, x, xs, w, (int8_t *)p.y, p.y_stride, s);
     else {
-        float *y = (float *)ws;
-        product(p, x, x_stride, xs, y, p.n, s);
+        float *y = (float *)take(p.rows * p.n * 4);
+        product_pairs(p, x, xs, w, y, p.n, s);
         if (p.y_scales) {
             quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
         } else {
@@ -366,6 +465,14 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
             count_launch();
         }
     }
+}
+
+int int8_device_error()
+{
+    int v = 0, z = 0;
+    SC_CUDA(cudaMemcpyFromSymbol(&v, tc::g_device_error, sizeof(int)));
+    if (v) SC_CUDA(cudaMemcpyToSymbol(tc::g_device_error, &z, sizeof(int)));
+    return v;
 }
 
 }  // namespace sc

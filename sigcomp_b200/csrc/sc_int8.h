@@ -25,6 +25,7 @@ struct Int8Linear {
     float *y_scales;            // int8 y: a scale for each row, or null
     float output_scale;         // int8 y without y_scales: the one scale
     void *workspace;
+    int x_packed, w_packed;     // addresses and strides are multiples of 16 bytes
 };
 
 void quantize_tokens(const void *x, int type, int64_t rows, int64_t cols, int64_t x_stride, int8_t *q, int64_t q_stride,

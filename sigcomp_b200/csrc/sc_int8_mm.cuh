@@ -1,0 +1,377 @@
+// Tensor-core products of the int8 operators.  Included by sc_int8.cu (one translation unit with its
+// device error flag).
+#pragma once
+
+namespace sc {
+namespace {
+
+using namespace tc;
+
+// ---- products on SM pairs ----------------------------------------------------------------------
+//
+// A unit is 256 rows x 256 channels: one tcgen05.mma (cta_group::2, M = 256, N = 256) per 32 bytes of
+// K over a pair of SMs, each holding its 128 rows of x and half of the weight rows of every K block
+// (128 bytes) in a ring of 32 KB stages that TMA fills.  Two accumulators of 256 TMEM columns let the
+// epilogue of one unit run under the products of the next.  Units go channel block by channel block
+// over the same rows, so that x comes from L2 after its first block.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (leader CTA), 2-9 epilogue (two for each TMEM lane quarter, half
+// of a unit's columns each).  Every warp of the epilogue keeps its own scales and bias and writes
+// its results through a 4 KB tile of its own, 32 rows of 128 bytes in the 128-byte swizzle, from which
+// TMA stores them: no warp waits for another, but for the row maximum of requantised rows.
+//
+// Requantised rows (REQUANT): a tile is 256 rows x all channels, at most the two accumulators' 512.
+// The first pass over a half turns its sums into results in 32 bits, puts them back into TMEM and takes
+// the row's maximum; the second, once both halves' maximum is known, scales and packs them.  The first
+// pass over half 0 runs under the products of half 1, the second over half 1 under those of the next
+// tile's half 0.
+//
+// Every wait is bounded; a warp that gives up ends, and the others end on their own limits.
+constexpr int PM = 128;                        // rows per CTA
+constexpr int PN = 256;                        // channels per unit
+constexpr int PK = 128;                        // bytes of K per stage
+constexpr int P_STAGES = 5;
+constexpr int P_A = PM * PK, P_B = (PN / 2) * PK, P_STAGE = P_A + P_B;
+constexpr int P_EPI = 8;
+constexpr int P_THREADS = 32 * (2 + P_EPI);
+constexpr int P_OFF_OUT = P_STAGES * P_STAGE;                      // staging: 4 KB per epilogue warp
+constexpr int P_OFF_TB = P_OFF_OUT + P_EPI * 4096;                 // {scale, bias} per warp and column
+constexpr int P_TB = 2 * (PN / 2) * 8;                             // two halves when requantising
+constexpr int P_OFF_MAX = P_OFF_TB + P_EPI * P_TB;                 // [2 parities][2 groups][128] row maxima
+constexpr int P_OFF_BAR = P_OFF_MAX + 2 * 2 * PM * 4;
+constexpr int P_NBAR = 2 * P_STAGES + 4 + 1;
+constexpr int P_OFF_CNT = P_OFF_BAR + P_NBAR * 8;                  // [8] row-maximum counters
+constexpr int P_OFF_TMEM = P_OFF_CNT + P_EPI * 4;
+constexpr int P_SMEM = P_OFF_TMEM + 16 + 1024;                     // + alignment slack
+static_assert(P_SMEM <= 232448, "shared memory per CTA");
+
+struct PairParams {
+    CUtensorMap x, w;                          // box 128 rows x 128 bytes
+    CUtensorMap y;                             // box 32 rows x 128 bytes
+    const float *xs, *ws, *bias;
+    int64_t rows;
+    int n, k, relu;
+    int y_tma;                                 // y is stored by TMA (16-byte aligned rows)
+    void *yp;
+    int64_t y_stride;
+    float *y_scales;
+};
+
+__device__ __forceinline__ void tma_store_2d(const void *tmap, const void *smem, int32_t x, int32_t y)
+{
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+                 ::"l"(tmap), "r"(smem_u32(smem)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// 32 sums of this thread's row -> results; tb: {scale, bias} of the columns
+__device__ __forceinline__ void affine32(const uint32_t (&v)[32], const float4 *tb, float s, int relu, float (&y)[32])
+{
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float4 c = tb[i];
+        y[2 * i] = __fmaf_rn(__fmul_rn(__int2float_rn((int32_t)v[2 * i]), s), c.x, c.y);
+        y[2 * i + 1] = __fmaf_rn(__fmul_rn(__int2float_rn((int32_t)v[2 * i + 1]), s), c.z, c.w);
+    }
+    if (relu) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) y[i] = max_nan(y[i], 0.0f);
+    }
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// This warp's 32 rows of 128 bytes from its staging tile to y: by TMA, which drops what lies beyond
+// the last row or column, or element by element where y's rows are not 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void store_tile(const PairParams &p, const uint8_t *tile, int64_t row0, int col0, int lane)
+{
+    constexpr int COLS = 128 / sizeof(T);
+    if (p.y_tma) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && row0 < p.rows && col0 < p.n) {
+            tma_store_2d(&p.y, tile, col0, (int32_t)row0);
+            bulk_commit();
+        }
+    } else {
+        __syncwarp();
+        const int nr = (int)min((int64_t)32, p.rows - row0);
+        for (int r = 0; r < nr; ++r)
+#pragma unroll
+            for (int c = lane; c < COLS; c += 32) {
+                const uint32_t off = c * (uint32_t)sizeof(T);
+                if (col0 + c < p.n)
+                    reinterpret_cast<T *>(p.yp)[(row0 + r) * p.y_stride + col0 + c] =
+                        *reinterpret_cast<const T *>(tile + sw128_offset(r, off >> 4) + (off & 15));
+            }
+        __syncwarp();
+    }
+}
+
+// the staging tile may be written again
+__device__ __forceinline__ void staging_free(const PairParams &p, int lane)
+{
+    if (p.y_tma && lane == 0) bulk_wait_read();
+    __syncwarp();
+}
+
+template <typename T, bool REQUANT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ PairParams p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = (uint64_t *)(smem + P_OFF_BAR), *empty = full + P_STAGES;
+    uint64_t *acc_full = empty + P_STAGES, *acc_empty = acc_full + 2, *drain = acc_empty + 2;
+    uint32_t *max_cnt = (uint32_t *)(smem + P_OFF_CNT);
+    uint32_t *tmem_slot = (uint32_t *)(smem + P_OFF_TMEM);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int nu = (p.n + PN - 1) / PN;                        // units per row tile
+    const int64_t units = (p.rows + 2 * PM - 1) / (2 * PM) * nu;
+    // this pair's units: every pairs-th, or, requantising, those of every pairs-th row tile
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int64_t group = REQUANT ? nu : 1;
+    const int nkb = (p.k + PK - 1) / PK;
+    const int last_k32 = (p.k - (nkb - 1) * PK + 31) / 32;     // 32-byte steps of the last K block
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < P_STAGES; ++s) {
+            mbar_init(&full[s], 1);                            // leader's producer (+ both CTAs' bytes)
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 2 * P_EPI);
+        }
+        mbar_init(drain, 1);
+        for (int i = 0; i < P_EPI; ++i) max_cnt[i] = 0;
+        fence_mbar_init();
+        prefetch_tmap(&p.x);
+        prefetch_tmap(&p.w);
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 2 * PN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                            // both CTAs' barriers exist
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int64_t g = pair * group; g < units && ok; g += pairs * group)
+                for (int64_t u = g; u < g + group && ok; ++u) {
+                    const int row0 = (int)(u / nu) * 2 * PM + (int)rank * PM;
+                    const int col0 = (int)(u % nu) * PN + (int)rank * (PN / 2);
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const int s = it % P_STAGES;
+                        if (!(ok = mbar_wait_cluster(&empty[s], ((it / P_STAGES) & 1) ^ 1))) break;
+                        uint8_t *st = smem + s * P_STAGE;
+                        const uint32_t fb = map_to_rank(&full[s], 0);
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * P_STAGE);
+                        tma_load_2d_pair(st, &p.x, fb, kb * PK, row0);
+                        tma_load_2d_pair(st + P_A, &p.w, fb, kb * PK, col0);
+                    }
+                }
+            if (!ok) {
+                // gave up: loads issued into this CTA may still land, see the fused kernels' abort path
+                for (uint32_t i = it > (uint32_t)P_STAGES ? it - P_STAGES : 0; i < it; ++i)
+                    mbar_wait_cluster_drain(rank == 0 ? &full[i % P_STAGES] : &empty[i % P_STAGES], (i / P_STAGES) & 1);
+                spin_ns(100000);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_i8(2 * PM, PN);
+            uint32_t it = 0, uu = 0;
+            bool ok = true;
+            for (int64_t g = pair * group; g < units && ok; g += pairs * group)
+                for (int64_t u = g; u < g + group && ok; ++u, ++uu) {
+                    const int ab = uu & 1;
+                    if (!(ok = mbar_wait_cluster(&acc_empty[ab], ((uu >> 1) & 1) ^ 1))) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + ab * PN;
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const int s = it % P_STAGES;
+                        if (!(ok = mbar_wait_cluster(&full[s], (it / P_STAGES) & 1))) break;
+                        tc_fence_after();
+                        const uint32_t a = smem_u32(smem + s * P_STAGE), b = a + P_A;
+                        const int steps = kb == nkb - 1 ? last_k32 : PK / 32;
+                        for (int i = 0; i < steps; ++i)
+                            mma_i8_pair(d, smem_desc_sw128(a + 32 * i), smem_desc_sw128(b + 32 * i), idesc,
+                                        (kb | i) ? 1u : 0u);
+                        mma_commit_pair(&empty[s], 0x3);
+                    }
+                    if (ok) mma_commit_pair(&acc_full[ab], 0x3);
+                }
+            mma_commit_pair(drain, 0x3);                       // completes after every MMA and commit above
+        }
+        __syncwarp();
+    } else {
+        const int q = warp & 3, grp = (warp - 2) >> 2;
+        uint8_t *tile = smem + P_OFF_OUT + (warp - 2) * 4096;
+        float2 *tb = (float2 *)(smem + P_OFF_TB + (warp - 2) * P_TB);
+        uint32_t *row_max = (uint32_t *)(smem + P_OFF_MAX);
+        const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16) + grp * (PN / 2);
+        uint32_t uu = 0, tiles = 0;
+        bool ok = true;
+        for (int64_t g = pair * group; g < units && ok; g += pairs * group, ++tiles) {
+            const int64_t row0 = g / nu * 2 * PM + rank * PM + q * 32;
+            const float s = row0 + lane < p.rows ? p.xs[row0 + lane] : 0.0f;
+            if (!REQUANT || tiles == 0) {
+                __syncwarp();
+                for (int h = 0; h < (REQUANT ? nu : 1); ++h) {
+                    const int c0 = (REQUANT ? h : (int)(g % nu)) * PN + grp * (PN / 2);
+#pragma unroll
+                    for (int i = 0; i < PN / 2; i += 32) {
+                        const int c = c0 + i + lane;
+                        tb[h * (PN / 2) + i + lane] =
+                            c < p.n ? make_float2(p.ws[c], p.bias ? p.bias[c] : 0.0f) : make_float2(0.0f, 0.0f);
+                    }
+                }
+                __syncwarp();
+            }
+            if constexpr (!REQUANT) {
+                const int ab = uu & 1;
+                const int col0 = (int)(g % nu) * PN + grp * (PN / 2);
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], (uu >> 1) & 1)))) break;
+                ++uu;
+                tc_fence_after();
+                constexpr int COLS = 128 / sizeof(T);          // columns of a staging tile
+#pragma unroll 1
+                for (int c = 0; c < PN / 2; c += COLS) {
+                    staging_free(p, lane);
+#pragma unroll
+                    for (int h = 0; h < COLS; h += 32) {
+                        uint32_t v[32];
+                        float y[32];
+                        tmem_ld32(lane_base + ab * PN + c + h, v);
+                        tmem_ld_wait();
+                        affine32(v, reinterpret_cast<const float4 *>(tb + c + h), s, p.relu, y);
+                        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<float4 *>(tile + sw128_offset(lane, j)) =
+                                    make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 8 + j)) =
+                                    make_uint4(pack2(y[8 * j], y[8 * j + 1], T()), pack2(y[8 * j + 2], y[8 * j + 3], T()),
+                                               pack2(y[8 * j + 4], y[8 * j + 5], T()),
+                                               pack2(y[8 * j + 6], y[8 * j + 7], T()));
+                        }
+                    }
+                    if (c + COLS == PN / 2) {                  // the accumulator's last columns are read
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
+                    }
+                    store_tile<T>(p, tile, row0, col0 + c, lane);
+                }
+            } else {
+                uint32_t top = 0;
+                for (int h = 0; h < nu && ok; ++h) {
+                    const int ab = (uu + h) & 1;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], ((uu + h) >> 1) & 1)))) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < PN / 2; c += 32) {
+                        uint32_t v[32];
+                        float y[32];
+                        tmem_ld32(lane_base + ab * PN + c, v);
+                        tmem_ld_wait();
+                        affine32(v, reinterpret_cast<const float4 *>(tb + h * (PN / 2) + c), s, p.relu, y);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            v[i] = __float_as_uint(y[i]);
+                            top = max(top, magnitude(y[i]));
+                        }
+                        tmem_st32(lane_base + ab * PN + c, v);
+                    }
+                    tmem_st_wait();
+                }
+                if (!ok) break;
+                // the row's other half of the columns is with the other warp of this quarter, which
+                // cannot be more than one tile ahead: two parities of the buffer are enough
+                uint32_t *mx = row_max + (tiles & 1) * 2 * PM;
+                mx[grp * PM + q * 32 + lane] = top;
+                __syncwarp();
+                if (lane == 0) counter_add_release(&max_cnt[grp * 4 + q], 1);
+                if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], tiles + 1)))) break;
+                top = max(top, mx[(grp ^ 1) * PM + q * 32 + lane]);
+                const RowScale rs = row_scale(top);
+                if (grp == 0 && row0 + lane < p.rows)
+                    p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                for (int h = 0; h < nu; ++h) {
+                    const int ab = (uu + h) & 1;
+                    staging_free(p, lane);
+#pragma unroll 1
+                    for (int c = 0; c < PN / 2; c += 32) {
+                        uint32_t v[32], o[8];
+                        tmem_ld32(lane_base + ab * PN + c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            o[i] = rs.finite ? pack4(quantise_bits(__uint_as_float(v[4 * i]), rs.r),
+                                                     quantise_bits(__uint_as_float(v[4 * i + 1]), rs.r),
+                                                     quantise_bits(__uint_as_float(v[4 * i + 2]), rs.r),
+                                                     quantise_bits(__uint_as_float(v[4 * i + 3]), rs.r))
+                                             : 0u;
+                        *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16 + 1)) =
+                            make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
+                    store_tile<int8_t>(p, tile, row0, h * PN + grp * (PN / 2), lane);
+                }
+                uu += nu;
+            }
+        }
+        if (p.y_tma && lane == 0) bulk_wait_all();
+        __syncwarp();
+    }
+    if (warp == 1) mbar_wait_cluster_drain(drain, 0);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();                                            // no CTA leaves while its peer may signal it
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem_base, 2 * PN);
+    }
+}
+
+}  // namespace
+}  // namespace sc

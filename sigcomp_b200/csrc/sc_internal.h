@@ -145,6 +145,11 @@ struct LayerDev {
 // a width other than 256 or 512, or a bias outside the range the digits reach (|b| <= 258,127).
 std::vector<int8_t> bias_tile(const int32_t *bias, int out_dim);
 
+// 2-D tensor map, rows `pitch` bytes apart, box = box_rows x box_cols elements (128 bytes a row), 128B
+// swizzle; elements outside read as zero and are not written.
+CUtensorMap tensor_map(const void *base, CUtensorMapDataType type, uint64_t cols, uint64_t rows, uint64_t pitch,
+                       uint32_t box_cols, uint32_t box_rows);
+
 // Launch the CUDA-core MLP: windows int16 [rows][window] -> logits int8 [rows][256].
 void mlp_simple(sc_model *m, const int16_t *windows, int64_t rows, int8_t *logits, cudaStream_t s);
 
@@ -183,6 +188,9 @@ void fused_compress(sc_model *m, const int32_t *tile_chunk, const int32_t *tile_
 void fused_decode(sc_model *m, const int64_t *order, int64_t n_rows, const int64_t *sorted_len,
                   const int64_t *lengths, DecState *state, const uint32_t *words, uint8_t *tokens_out,
                   const int64_t *out_off, uint8_t *errors, cudaStream_t s);
+
+// Clears and returns the error flag that a timed-out wait of the int8 operators set on the current device.
+int int8_device_error();
 
 // Value of the device error flag set by timed-out waits (optionally cleared).
 int read_device_error(int clear);

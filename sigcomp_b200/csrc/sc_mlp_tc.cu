@@ -363,19 +363,25 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
 // 2-D int8 tensor [rows][cols] (row pitch `pitch` bytes), box = box_rows x 128 bytes, 128B swizzle
 CUtensorMap make_tmap(const void *base, uint64_t cols, uint64_t rows, uint64_t pitch, uint32_t box_rows)
 {
+    return tensor_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, cols, rows, pitch, KB, box_rows);
+}
+
+}  // namespace
+
+CUtensorMap tensor_map(const void *base, CUtensorMapDataType type, uint64_t cols, uint64_t rows, uint64_t pitch,
+                       uint32_t box_cols, uint32_t box_rows)
+{
     CUtensorMap m;
     cuuint64_t dims[2] = {cols, rows};
     cuuint64_t strides[1] = {pitch};
-    cuuint32_t box[2] = {(cuuint32_t)KB, box_rows};
+    cuuint32_t box[2] = {box_cols, box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+    CUresult r = encode_fn()(&m, type, 2, const_cast<void *>(base), dims, strides, box, estr,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw CudaError{cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed"};
     return m;
 }
-
-}  // namespace
 
 std::vector<int8_t> bias_tile(const int32_t *bias, int out_dim)
 {

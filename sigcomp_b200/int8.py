@@ -129,8 +129,12 @@ def dequantize_tokens(q, scales, dtype=torch.float32):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(x_type, x_stride, w_stride, rows, n, k, y_type):
-    return _lib.load().sc_int8_linear_workspace(x_type, x_stride, w_stride, rows, n, k, y_type)
+def _workspace_bytes(*sizes):
+    return _lib.load().sc_int8_linear_workspace(*sizes)
+
+
+def _packed(t, stride, k):
+    return t.data_ptr() % 16 == 0 and stride % 16 == 0 and stride >= k
 
 
 def _linear(x, x_scales, weight, weight_scales, bias, relu, y_type, output_scale):
@@ -169,7 +173,7 @@ def _linear(x, x_scales, weight, weight_scales, bias, relu, y_type, output_scale
         y = torch.empty((m, n), dtype=y_type, device=device)
     xt, yt = _TYPES[x.dtype], _TYPES[y_type]
     x_stride, w_stride = rows.stride(0), max(weight.stride(0), k)
-    size = _workspace_bytes(xt, x_stride, w_stride, m, n, k, yt)
+    size = _workspace_bytes(xt, _packed(rows, x_stride, k), _packed(weight, w_stride, k), m, n, k, yt, y_scales is not None)
     work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
     _lib.check(_lib.load().sc_int8_linear_device(
         device.index, rows.data_ptr(), xt, x_stride, None if x_scales is None else x_scales.data_ptr(),
@@ -212,3 +216,10 @@ def int8_linear_requant(q, scales, weight, weight_scales, bias=None, *, relu=Fal
             raise ValueError("output_scale must be a finite positive number")
     y, y_scales = _linear(q, scales, weight, weight_scales, bias, relu, torch.int8, output_scale)
     return y if y_scales is None else (y, y_scales)
+
+
+def check_waits(device=None):
+    """Wait for the current stream of ``device`` and raise if a kernel of these operators gave up a wait
+    there (2 s, see ``sc_int8_status_device``) since the last such check."""
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    _lib.check(_lib.load().sc_int8_status_device(device.index or 0, _stream(device)), "sc_int8_status_device")

@@ -97,7 +97,7 @@ def test_c_entry_points_do_nothing_for_no_rows():
     L = _lib.load()
     assert L.sc_quantize_tokens_device(0, None, 0, 0, 5, 5, None, 5, None, None) == _lib.SC_OK
     assert L.sc_dequantize_tokens_device(0, None, 5, None, 1.0, 0, 5, None, 0, 5, None) == _lib.SC_OK
-    assert L.sc_int8_linear_workspace(0, 32, 32, 0, 8, 32, 3) == 0
+    assert L.sc_int8_linear_workspace(0, 1, 1, 0, 8, 32, 3, 1) == 0
 
 
 @pytest.mark.parametrize("args", [
@@ -123,5 +123,5 @@ def test_dequantise_entry_point_refuses(args):
 
 
 def test_workspace_size_is_a_whole_number_of_bytes():
-    assert isinstance(_lib.load().sc_int8_linear_workspace(1, 8192, 8192, 1, 512, 8192, 2), int)
+    assert isinstance(_lib.load().sc_int8_linear_workspace(1, 1, 1, 1, 512, 8192, 2, 0), int)
     assert ctypes.sizeof(ctypes.c_int64) == 8
