@@ -236,6 +236,14 @@ k_product_any(const int8_t *__restrict__ x, int64_t x_stride, const float *__res
         }
 }
 
+// sat(rint(y / scale)) in the low byte; a NaN becomes 0
+__device__ __forceinline__ uint32_t static_bits(float y, float scale)
+{
+    int32_t o;
+    asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(o) : "f"(__fdiv_rn(y, scale)));
+    return (uint32_t)o & 0xffu;
+}
+
 }  // namespace
 }  // namespace sc
 
@@ -245,19 +253,6 @@ namespace sc {
 namespace {
 
 // ---- host side -------------------------------------------------------------------------------
-
-// Rows in 32 bits to int8 by one given scale: sat(rint(y / scale)); a NaN becomes 0.
-__global__ void __launch_bounds__(256)
-k_static(const float *__restrict__ y, int64_t rows, int cols, float scale, int8_t *__restrict__ q, int64_t q_stride)
-{
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    for (int c = threadIdx.x & 31; c < cols; c += 32) {
-        int32_t o;
-        asm("cvt.rni.sat.s8.f32 %0, %1;" : "=r"(o) : "f"(__fdiv_rn(y[row * cols + c], scale)));
-        q[row * q_stride + c] = (int8_t)o;
-    }
-}
 
 // Rows copied to a multiple of 16 bytes apart, for arrays that TMA cannot read as they lie.  Bytes behind
 // a row's end stay as they are: the tensor map ends with the row.
@@ -360,12 +355,11 @@ template <> constexpr CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_
 template <> constexpr CUtensorMapDataType map_type<int8_t>() { return CU_TENSOR_MAP_DATA_TYPE_UINT8; }
 
 // y (T; int8: requantised with a scale for each row, at most 512 channels) of int8 rows, on SM pairs
-template <typename T>
+template <typename T, int MODE>
 void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, cudaStream_t s)
 {
-    constexpr bool REQUANT = sizeof(T) == 1;
     static std::atomic<uint64_t> ready{0};
-    allow_smem(k_pair<T, REQUANT>, P_SMEM, ready);
+    allow_smem(k_pair<T, MODE>, P_SMEM, ready);
     PairParams a;
     a.x = tensor_map(x.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.rows, x.stride, PK, PM);
     a.w = tensor_map(w.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.n, w.stride, PK, PN / 2);
@@ -381,13 +375,54 @@ void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y,
     a.yp = y;
     a.y_stride = y_stride;
     a.y_scales = p.y_scales;
+    a.output_scale = p.output_scale;
     const int64_t tiles = (p.rows + 2 * PM - 1) / (2 * PM), units = (p.n + PN - 1) / PN;
-    const int64_t work = REQUANT ? tiles : tiles * units;
+    const int64_t work = MODE == ROWS ? tiles : tiles * units;
     const unsigned pairs = (unsigned)std::min<int64_t>(work, sm_count() / 2);
-    k_pair<T, REQUANT><<<2 * pairs, P_THREADS, P_SMEM, s>>>(a);
+    k_pair<T, MODE><<<2 * pairs, P_THREADS, P_SMEM, s>>>(a);
     SC_LAUNCH_CHECK();
     count_launch();
 }
+
+// y (float types, or int8 by one scale) of few int8 rows; `bt` tokens per tile, K split over `split` CTAs
+template <int BT>
+void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride, int split,
+                 cudaStream_t s)
+{
+    using C = FewCfg<BT>;
+    static std::atomic<uint64_t> ready{0};
+    allow_smem(k_few<BT>, C::SMEM, ready);
+    FewParams a;
+    a.w = tensor_map(w.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.n, w.stride, PK, 128);
+    a.x = tensor_map(x.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.rows, x.stride, PK, BT);
+    a.xs = xs;
+    a.ws = p.w_scales;
+    a.bias = p.bias;
+    a.rows = p.rows;
+    a.n = (int)p.n;
+    a.k = (int)p.k;
+    a.relu = p.relu;
+    a.y_type = y_type;
+    a.y = y;
+    a.y_stride = y_stride;
+    a.output_scale = p.output_scale;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)split, (unsigned)((p.n + 127) / 128), (unsigned)((p.rows + BT - 1) / BT));
+    cfg.blockDim = dim3(F_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    SC_CUDA(cudaLaunchKernelEx(&cfg, k_few<BT>, a));
+    count_launch();
+}
+
+// Whether the pair kernel's units leave SM pairs without work.
+bool few(int64_t rows, int64_t n) { return (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN) < 64; }
 
 int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
@@ -411,7 +446,30 @@ void dequantize_tokens(const int8_t *q, int64_t q_stride, const float *scales, f
 
 // Workspace: the rows of a float x held in 8 bits and their scales, x and w spread where TMA cannot read
 // them, and the product's rows in 32 bits where they come back quantised by a launch of their own.
-static bool own_requant(const Int8Linear &p) { return p.y_type == SC_TYPE_I8 && !(p.y_scales && p.n <= 2 * PN); }
+static bool own_requant(const Int8Linear &p)
+{
+    return p.y_type == SC_TYPE_I8 && p.y_scales && (p.n > 2 * PN || few(p.rows, p.n));
+}
+
+static void product(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride,
+                    cudaStream_t s)
+{
+    const bool rows = y_type == SC_TYPE_I8 && p.y_scales;
+    if (!rows && few(p.rows, p.n)) {
+        const int64_t nkb = (p.k + PK - 1) / PK;
+        const int bt = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
+        const int64_t tiles = (p.rows + bt - 1) / bt * ((p.n + 127) / 128);
+        int split = 1;
+        while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * tiles <= sm_count()) split *= 2;
+        if (bt == 16) product_few<16>(p, x, xs, w, y, y_type, y_stride, split, s);
+        else if (bt == 32) product_few<32>(p, x, xs, w, y, y_type, y_stride, split, s);
+        else product_few<64>(p, x, xs, w, y, y_type, y_stride, split, s);
+    } else if (rows) product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, y_stride, s);
+    else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, y_stride, s);
+    else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, y_stride, s);
+    else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, y_stride, s);
+    else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, s);
+}
 
 int64_t int8_linear_workspace(const Int8Linear &p)
 {
@@ -450,20 +508,12 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
         x = spread(x.p, p.rows, x.stride);
     }
     if (!p.w_packed) w = spread(p.w, p.n, p.w_stride);
-    if (p.y_type == SC_TYPE_F32) product_pairs(p, x, xs, w, (float *)p.y, p.y_stride, s);
-    else if (p.y_type == SC_TYPE_F16) product_pairs(p, x, xs, w, (__half *)p.y, p.y_stride, s);
-    else if (p.y_type == SC_TYPE_BF16) product_pairs(p, x, xs, w, (__nv_bfloat16 *)p.y, p.y_stride, s);
-    else if (!own_requant(p)) product_pairs(p, x, xs, w, (int8_t *)p.y, p.y_stride, s);
-    else {
+    if (own_requant(p)) {
         float *y = (float *)take(p.rows * p.n * 4);
-        product_pairs(p, x, xs, w, y, p.n, s);
-        if (p.y_scales) {
-            quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
-        } else {
-            k_static<<<grid_x((p.rows + 7) / 8), 256, 0, s>>>(y, p.rows, (int)p.n, p.output_scale, (int8_t *)p.y, p.y_stride);
-            SC_LAUNCH_CHECK();
-            count_launch();
-        }
+        product(p, x, xs, w, y, SC_TYPE_F32, p.n, s);
+        quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+    } else {
+        product(p, x, xs, w, p.y, p.y_type, p.y_stride, s);
     }
 }
 

@@ -45,6 +45,9 @@ constexpr int P_OFF_TMEM = P_OFF_CNT + P_EPI * 4;
 constexpr int P_SMEM = P_OFF_TMEM + 16 + 1024;                     // + alignment slack
 static_assert(P_SMEM <= 232448, "shared memory per CTA");
 
+// what becomes of the results in 32 bits: rounded to T, quantised row by row, or by one scale
+enum { PLAIN, ROWS, STATIC };
+
 struct PairParams {
     CUtensorMap x, w;                          // box 128 rows x 128 bytes
     CUtensorMap y;                             // box 32 rows x 128 bytes
@@ -55,6 +58,7 @@ struct PairParams {
     void *yp;
     int64_t y_stride;
     float *y_scales;
+    float output_scale;
 };
 
 __device__ __forceinline__ void tma_store_2d(const void *tmap, const void *smem, int32_t x, int32_t y)
@@ -78,6 +82,9 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // 32 sums of this thread's row -> results; tb: {scale, bias} of the columns
 __device__ __forceinline__ void affine32(const uint32_t (&v)[32], const float4 *tb, float s, int relu, float (&y)[32])
@@ -140,9 +147,10 @@ __device__ __forceinline__ void staging_free(const PairParams &p, int lane)
     __syncwarp();
 }
 
-template <typename T, bool REQUANT>
+template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ PairParams p)
 {
+    constexpr bool REQUANT = MODE == ROWS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = (uint64_t *)(smem + P_OFF_BAR), *empty = full + P_STAGES;
@@ -278,7 +286,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair
                         tmem_ld32(lane_base + ab * PN + c + h, v);
                         tmem_ld_wait();
                         affine32(v, reinterpret_cast<const float4 *>(tb + c + h), s, p.relu, y);
-                        if constexpr (sizeof(T) == 4) {
+                        if constexpr (MODE == STATIC) {
+                            uint32_t o[8];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                o[j] = pack4(static_bits(y[4 * j], p.output_scale), static_bits(y[4 * j + 1], p.output_scale),
+                                             static_bits(y[4 * j + 2], p.output_scale),
+                                             static_bits(y[4 * j + 3], p.output_scale));
+                            *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 16)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 16 + 1)) =
+                                make_uint4(o[4], o[5], o[6], o[7]);
+                        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
                                 *reinterpret_cast<float4 *>(tile + sw128_offset(lane, j)) =
@@ -370,6 +389,183 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, 2 * PN);
+    }
+}
+
+// ---- products of a few tokens, K split over a cluster -------------------------------------------
+//
+// With few rows the weights are what has to be read, so they take the side of the MMA that is always
+// full: a CTA computes 128 channels (M) x BT tokens (N = 16, 32, 64 or 128), and where such tiles are fewer
+// than the SMs a cluster of up to eight CTAs splits the tile's K.  Each CTA then owns BT / S of the tokens:
+// the others put their whole sums for them into its shared memory, 128 channels at a time, one
+// cluster barrier publishes them, and the owner adds the S parts (whole numbers: any order) and writes
+// the results, neighbouring lanes writing neighbouring channels.  No workspace, no counters, one launch.
+//
+// Warps: 0 TMA producer, 1 MMA issuer, 2-5 epilogue (one for each TMEM lane quarter).
+struct FewParams {
+    CUtensorMap w, x;                          // boxes 128 and BT rows x 128 bytes
+    const float *xs, *ws, *bias;
+    int64_t rows;
+    int n, k, relu, y_type;
+    void *y;
+    int64_t y_stride;
+    float output_scale;
+};
+
+__device__ __forceinline__ void store_one(void *y, int type, int64_t at, float v, float output_scale)
+{
+    if (type == SC_TYPE_F32) reinterpret_cast<float *>(y)[at] = v;
+    else if (type == SC_TYPE_F16) reinterpret_cast<__half *>(y)[at] = __float2half_rn(v);
+    else if (type == SC_TYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
+    else reinterpret_cast<int8_t *>(y)[at] = (int8_t)static_bits(v, output_scale);
+}
+
+constexpr int F_THREADS = 192;
+constexpr int F_MAX_SPLIT = 8;
+
+template <int BT>
+struct FewCfg {
+    static constexpr int STAGES = BT <= 32 ? 9 : BT == 64 ? 7 : 4;
+    static constexpr int STAGE = 128 * PK + BT * PK;
+    static constexpr int OFF_RECV = STAGES * STAGE;                    // [S][BT / S][128] sums of the owned tokens
+    static constexpr int OFF_BAR = OFF_RECV + BT * 128 * 4;
+    static constexpr int OFF_TMEM = OFF_BAR + (2 * STAGES + 1) * 8;
+    static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+    static constexpr int TMEM = BT < 32 ? 32 : BT;
+    static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+
+template <int BT>
+__global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ FewParams p)
+{
+    using C = FewCfg<BT>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + C::STAGES, *done = empty + C::STAGES;
+    uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_TMEM);
+    int32_t *recv = (int32_t *)(smem + C::OFF_RECV);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = gridDim.x;                                           // the cluster: x is the split
+    const int part = blockIdx.x;
+    const int c0 = blockIdx.y * 128;
+    const int64_t t0 = (int64_t)blockIdx.z * BT;
+    const int nkb_all = (p.k + PK - 1) / PK;
+    const int kb0 = (int)((int64_t)nkb_all * part / S), kb1 = (int)((int64_t)nkb_all * (part + 1) / S);
+    const int last_k32 = (p.k - (nkb_all - 1) * PK + 31) / 32;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        fence_mbar_init();
+        prefetch_tmap(&p.w);
+        prefetch_tmap(&p.x);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, C::TMEM);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (S > 1) cluster_arrive();                                       // this CTA runs: its memory may be written
+    const uint32_t tmem = *tmem_slot;
+
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::STAGES;
+                if (!(ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1))) break;
+                uint8_t *st = smem + s * C::STAGE;
+                mbar_arrive_expect_tx(&full[s], C::STAGE);
+                tma_load_2d(st, &p.w, &full[s], kb * PK, c0);
+                tma_load_2d(st + 128 * PK, &p.x, &full[s], kb * PK, (int)t0);
+            }
+            if (!ok) {                                                 // loads still landing, then end
+                for (uint32_t i = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+                    mbar_wait_cluster_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
+                spin_ns(100000);
+            }
+        }
+        __syncwarp();
+        if (S > 1) cluster_wait();
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_i8(128, BT);
+            uint32_t it = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int s = it % C::STAGES;
+                if (!(ok = mbar_wait(&full[s], (it / C::STAGES) & 1))) break;
+                tc_fence_after();
+                const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + 128 * PK;
+                const int steps = kb == nkb_all - 1 ? last_k32 : PK / 32;
+                for (int i = 0; i < steps; ++i)
+                    mma_i8(tmem, smem_desc_sw128(a + 32 * i), smem_desc_sw128(b + 32 * i), idesc, (it | i) ? 1u : 0u);
+                mma_commit(&empty[s]);
+            }
+            mma_commit(done);                                          // after every MMA above, given up or not
+        }
+        __syncwarp();
+        if (S > 1) cluster_wait();
+    } else {
+        // this thread's channel; tokens are the columns
+        const int q = warp & 3, ch = c0 + q * 32 + lane;
+        const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
+        mbar_wait(done, 0);
+        __syncwarp();
+        if (S > 1) cluster_wait();
+        tc_fence_after();
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+        const int own = BT / S;                                        // S is a power of two, at most BT / 2
+#pragma unroll 1
+        for (int j0 = 0; j0 < BT; j0 += 16) {
+            if (t0 + j0 >= p.rows) break;
+            uint32_t v[16];
+            tmem_ld16(taddr + j0, v);
+            tmem_ld_wait();
+            if (S == 1) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int64_t r = t0 + j0 + j;
+                    if (r < p.rows && ch < p.n)
+                        store_one(p.y, p.y_type, r * p.y_stride + ch, affine((int32_t)v[j], p.xs[r], t, b, p.relu),
+                                  p.output_scale);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int col = j0 + j;
+                    const uint32_t at = map_to_rank(recv + (part * own + col % own) * 128 + q * 32 + lane, col / own);
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (S > 1) {
+        cluster_sync();                                                // every CTA's sums are where they belong
+        if (warp >= 2) {
+            const int q = warp & 3, ch = c0 + q * 32 + lane;
+            const int own = BT / S;
+            const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
+            for (int j = 0; j < own; ++j) {
+                const int64_t r = t0 + part * own + j;
+                if (r >= p.rows || ch >= p.n) break;
+                int32_t sum = 0;
+                for (int i = 0; i < S; ++i) sum += recv[(i * own + j) * 128 + q * 32 + lane];
+                store_one(p.y, p.y_type, r * p.y_stride + ch, affine(sum, p.xs[r], t, b, p.relu), p.output_scale);
+            }
+        }
+    }
+    if (warp == 1) {
+        mbar_wait_cluster_drain(done, 0);
+        tc_fence_after();
+        tmem_dealloc(tmem, C::TMEM);
     }
 }
 
