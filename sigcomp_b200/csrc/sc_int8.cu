@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <type_traits>
 
 #include "sc_internal.h"
 #include "sc_int8.h"
@@ -68,66 +69,122 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// A vector of 16 bytes of a row, kept as it was read: the row is converted where it is used, which
+// halves the registers of 16-bit types and takes their magnitudes two at a time.
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ uint32_t top(const uint4 &r, uint32_t m)
+    {
+        return max(max(m, max(r.x & 0x7fffffffu, r.y & 0x7fffffffu)), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t m) { return m; }
+    static __device__ __forceinline__ void quantise(const uint4 &v, float r, uint32_t (&o)[1])
+    {
+        o[0] = pack4(quantise_bits(__uint_as_float(v.x), r), quantise_bits(__uint_as_float(v.y), r),
+                     quantise_bits(__uint_as_float(v.z), r), quantise_bits(__uint_as_float(v.w), r));
+    }
+};
+template <typename T> struct Vec16 {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ uint32_t top(const uint4 &r, uint32_t m)
+    {
+        m = __vmaxu2(m, __vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu));
+        return __vmaxu2(m, __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+    }
+    static __device__ __forceinline__ uint32_t top_bits(uint32_t m)
+    {
+        const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+        return __float_as_uint(to_f32<T>(*reinterpret_cast<const T *>(&h)));
+    }
+    static __device__ __forceinline__ void quantise(const uint4 &v, float r, uint32_t (&o)[2])
+    {
+        const T *e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            o[i] = pack4(quantise_bits(to_f32<T>(e[4 * i]), r), quantise_bits(to_f32<T>(e[4 * i + 1]), r),
+                         quantise_bits(to_f32<T>(e[4 * i + 2]), r), quantise_bits(to_f32<T>(e[4 * i + 3]), r));
+    }
+};
+template <> struct Vec<__half> : Vec16<__half> {};
+template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
+
+// columns c .. c + N of a row of `cols`, zeros behind its end; ALIGNED: rows start on 16 bytes
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ uint4 load_vec(const T *row, int c, int cols)
+{
+    constexpr int N = Vec<T>::N;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (ALIGNED && c + N <= cols) {
+        raw = *reinterpret_cast<const uint4 *>(row + c);
+    } else {
+        T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < cols) e[i] = row[c + i];
+    }
+    return raw;
+}
+
 // ---- quantise --------------------------------------------------------------------------------
-// A row is read once: T threads hold its 16-byte vectors in registers through the maximum.
-// Bound by HBM (e + 1 bytes per element).
-template <typename T, int THREADS, int HELD, bool ALIGNED>
+// A row is read once: T threads hold its 16-byte vectors in registers through the maximum, and a group
+// of threads holds R rows at a time where rows are short, so that enough loads are in flight.  Bound by
+// HBM (e + 1 bytes per element).
+template <typename T, int THREADS, int HELD, int R, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ q, int64_t q_stride,
            float *__restrict__ scales)
 {
-    constexpr int V = 16 / sizeof(T);
-    constexpr int PER_BLOCK = THREADS < 256 ? 256 / THREADS : 1;
-    __shared__ uint32_t tops[32];
-    const int t = threadIdx.x % THREADS;
-    const int64_t row = (int64_t)blockIdx.x * PER_BLOCK + threadIdx.x / THREADS;
-    if (THREADS <= 32 && row >= rows) return;        // whole warps: THREADS divides 32's multiples
-    const T *xr = x + row * x_stride;
-    float v[HELD][V];
-    uint32_t top = 0;
+    constexpr int N = Vec<T>::N;
+    constexpr int GROUPS = THREADS < 256 ? 256 / THREADS : 1;      // of THREADS threads, R rows each
+    __shared__ uint32_t tops[R][32];
+    const int t = threadIdx.x % THREADS, grp = threadIdx.x / THREADS;
+    const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + grp) * R;
+    uint4 v[R][HELD];
+    uint32_t top[R];
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        const int c = (h * THREADS + t) * V;
-        if (ALIGNED && c + V <= cols) {
-            const uint4 raw = *reinterpret_cast<const uint4 *>(xr + c);
-            const T *e = reinterpret_cast<const T *>(&raw);
+    for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[h][i] = to_f32<T>(e[i]);
-        } else {
+        for (int h = 0; h < HELD; ++h)
+            v[i][h] = row0 + i < rows ? load_vec<T, ALIGNED>(x + (row0 + i) * x_stride, (h * THREADS + t) * N, cols)
+                                      : make_uint4(0, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) v[h][i] = c + i < cols ? to_f32<T>(xr[c + i]) : 0.0f;
-        }
+    for (int i = 0; i < R; ++i) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) m = Vec<T>::top(v[i][h], m);
+        top[i] = __reduce_max_sync(0xffffffffu, Vec<T>::top_bits(m));
+        if (THREADS > 32 && (threadIdx.x & 31) == 0) tops[i][threadIdx.x >> 5] = top[i];
     }
-#pragma unroll
-    for (int h = 0; h < HELD; ++h)
-#pragma unroll
-        for (int i = 0; i < V; ++i) top = max(top, magnitude(v[h][i]));
-    top = __reduce_max_sync(0xffffffffu, top);
     if (THREADS > 32) {
-        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
         __syncthreads();
         const int w = threadIdx.x & 31;
-        top = __reduce_max_sync(0xffffffffu, w < THREADS / 32 ? tops[w] : 0u);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+            top[i] = __reduce_max_sync(0xffffffffu, w < THREADS / 32 ? tops[i][grp * (THREADS / 32) + w] : 0u);
     }
-    const RowScale rs = row_scale(top);
-    if (t == 0) scales[row] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
-    int8_t *qr = q + row * q_stride;
 #pragma unroll
-    for (int h = 0; h < HELD; ++h) {
-        const int c = (h * THREADS + t) * V;
-        uint32_t p[V / 4];
+    for (int i = 0; i < R; ++i) {
+        if (row0 + i >= rows) break;
+        const RowScale rs = row_scale(top[i]);
+        if (t == 0) scales[row0 + i] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+        int8_t *qr = q + (row0 + i) * q_stride;
 #pragma unroll
-        for (int i = 0; i < V / 4; ++i)
-            p[i] = rs.finite ? pack4(quantise_bits(v[h][4 * i], rs.r), quantise_bits(v[h][4 * i + 1], rs.r),
-                                     quantise_bits(v[h][4 * i + 2], rs.r), quantise_bits(v[h][4 * i + 3], rs.r))
-                             : 0u;
-        if (ALIGNED && c + V <= cols) {
-            if (V == 8) *reinterpret_cast<uint2 *>(qr + c) = make_uint2(p[0], p[V / 4 - 1]);
-            else *reinterpret_cast<uint32_t *>(qr + c) = p[0];
-        } else {
+        for (int h = 0; h < HELD; ++h) {
+            const int c = (h * THREADS + t) * N;
+            uint32_t o[N / 4];
+            Vec<T>::quantise(v[i][h], rs.r, o);
+            if (!rs.finite)
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (c + i < cols) qr[c + i] = (int8_t)(p[i / 4] >> (8 * (i % 4)));
+                for (int j = 0; j < N / 4; ++j) o[j] = 0;
+            if (ALIGNED && c + N <= cols) {
+                if constexpr (N == 8) *reinterpret_cast<uint2 *>(qr + c) = make_uint2(o[0], o[1]);
+                else *reinterpret_cast<uint32_t *>(qr + c) = o[0];
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (c + j < cols) qr[c + j] = (int8_t)(o[j / 4] >> (8 * (j % 4)));
+            }
         }
     }
 }
@@ -141,7 +198,7 @@ k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__r
     __shared__ uint32_t tops[32];
     const T *xr = x + (int64_t)blockIdx.x * x_stride;
     uint32_t top = 0;
-    for (int c = threadIdx.x; c < cols; c += 1024) top = max(top, magnitude(to_f32<T>(xr[c])));
+    for (int64_t c = threadIdx.x; c < cols; c += 1024) top = max(top, magnitude(to_f32<T>(xr[c])));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
     __syncthreads();
@@ -149,35 +206,55 @@ k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__r
     const RowScale rs = row_scale(top);
     if (threadIdx.x == 0) scales[blockIdx.x] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
     int8_t *qr = q + (int64_t)blockIdx.x * q_stride;
-    for (int c = threadIdx.x; c < cols; c += 1024)
+    for (int64_t c = threadIdx.x; c < cols; c += 1024)
         qr[c] = rs.finite ? (int8_t)quantise_bits(to_f32<T>(xr[c]), rs.r) : 0;
 }
 
 // ---- dequantise ------------------------------------------------------------------------------
-// One warp per 512 columns of a row, 16 values a thread.  Bound by HBM (1 + e bytes per element).
+// 16 bytes of results a thread and row, four rows in flight: a block's 256 threads are 2^log_lanes
+// vectors wide.  Bound by HBM (1 + e bytes per element).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
 k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__restrict__ scales, float scale, int64_t rows,
-             int cols, T *__restrict__ y, int64_t y_stride)
+             int cols, T *__restrict__ y, int64_t y_stride, int log_lanes)
 {
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= rows) return;
-    const float s = scales ? scales[row] : scale;
-    const int8_t *qr = q + row * q_stride;
-    T *yr = y + row * y_stride;
-    for (int64_t c0 = (int64_t)blockIdx.y * 512; c0 < cols; c0 += (int64_t)gridDim.y * 512) {
-        const int c = (int)c0 + (threadIdx.x & 31) * 16;
-        if (ALIGNED && c + 16 <= cols) {
-            const uint4 raw = *reinterpret_cast<const uint4 *>(qr + c);
-            const int8_t *e = reinterpret_cast<const int8_t *>(&raw);
-            __align__(16) T out[16];
+    constexpr int N = Vec<T>::N, U = 4;
+    const int deep = 256 >> log_lanes;                             // rows of one pass
+    const int64_t row0 = (int64_t)blockIdx.x * deep * U + (threadIdx.x >> log_lanes);
+    const int lane = threadIdx.x & ((1 << log_lanes) - 1);
+    for (int64_t c64 = ((int64_t)blockIdx.y << log_lanes) * N; c64 < cols; c64 += ((int64_t)gridDim.y << log_lanes) * N) {
+        const int c = (int)c64 + lane * N;
+        if (c >= cols) break;
+        if (ALIGNED && c + N <= cols) {
+            uint2 raw[U];
+            float s[U];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) out[i] = from_f32<T>(__fmul_rn((float)e[i], s));
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = row0 + u * deep;
+                if (r >= rows) break;
+                const int8_t *at = q + r * q_stride + c;
+                if constexpr (N == 8) raw[u] = *reinterpret_cast<const uint2 *>(at);
+                else raw[u].x = *reinterpret_cast<const uint32_t *>(at);
+                s[u] = scales ? scales[r] : scale;
+            }
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T); ++i)
-                reinterpret_cast<uint4 *>(yr + c)[i] = reinterpret_cast<const uint4 *>(out)[i];
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = row0 + u * deep;
+                if (r >= rows) break;
+                const int8_t *e = reinterpret_cast<const int8_t *>(&raw[u]);
+                __align__(16) T out[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) out[i] = from_f32<T>(__fmul_rn((float)e[i], s[u]));
+                *reinterpret_cast<uint4 *>(y + r * y_stride + c) = *reinterpret_cast<const uint4 *>(out);
+            }
         } else {
-            for (int i = 0; i < 16 && c + i < cols; ++i) yr[c + i] = from_f32<T>(__fmul_rn((float)qr[c + i], s));
+            for (int u = 0; u < U; ++u) {
+                const int64_t r = row0 + u * deep;
+                if (r >= rows) break;
+                const float s = scales ? scales[r] : scale;
+                for (int i = 0; i < N && c + i < cols; ++i)
+                    y[r * y_stride + c + i] = from_f32<T>(__fmul_rn((float)q[r * q_stride + c + i], s));
+            }
         }
     }
 }
@@ -248,6 +325,7 @@ __device__ __forceinline__ uint32_t static_bits(float y, float scale)
 }  // namespace sc
 
 #include "sc_int8_mm.cuh"
+#include "sc_int8_token.cuh"
 
 namespace sc {
 namespace {
@@ -282,48 +360,6 @@ unsigned grid_x(int64_t blocks)
     return (unsigned)blocks;
 }
 
-template <typename T>
-void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t qs, float *scales, cudaStream_t s)
-{
-    constexpr int V = 16 / sizeof(T);
-    const bool al = aligned(x, xs * (int64_t)sizeof(T), 16) && aligned(q, qs, V);
-#define SC_Q(THREADS, HELD)                                                                                        \
-    do {                                                                                                           \
-        const unsigned g = grid_x(THREADS < 256 ? (rows + 256 / THREADS - 1) / (256 / THREADS) : rows);            \
-        if (al) k_quantize<T, THREADS, HELD, true><<<g, THREADS < 256 ? 256 : THREADS, 0, s>>>(x, rows, cols, xs, q, qs, scales); \
-        else k_quantize<T, THREADS, HELD, false><<<g, THREADS < 256 ? 256 : THREADS, 0, s>>>(x, rows, cols, xs, q, qs, scales);   \
-    } while (0)
-    if (cols <= 32 * V) SC_Q(32, 1);
-    else if (cols <= 64 * V) SC_Q(32, 2);
-    else if (cols <= 128 * V) SC_Q(32, 4);
-    else if (cols <= 256 * V) SC_Q(256, 1);
-    else if (cols <= 512 * V) SC_Q(256, 2);
-    else if (cols <= 1024 * V) SC_Q(1024, 1);
-    else if (cols <= 4096 * V) SC_Q(1024, 4);
-    else k_quantize_long<T><<<grid_x(rows), 1024, 0, s>>>(x, cols, xs, q, qs, scales);
-#undef SC_Q
-    SC_LAUNCH_CHECK();
-    count_launch();
-}
-
-template <typename T>
-void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, int64_t rows, int cols, T *y, int64_t ys,
-                cudaStream_t s)
-{
-    const dim3 g(grid_x((rows + 7) / 8), (unsigned)std::min((cols + 511) / 512, 65535));
-    if (aligned(q, qs, 16) && aligned(y, ys * (int64_t)sizeof(T), 16))
-        k_dequantize<T, true><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys);
-    else
-        k_dequantize<T, false><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys);
-    SC_LAUNCH_CHECK();
-    count_launch();
-}
-
-struct Rows8 {
-    const int8_t *p;
-    int64_t stride;
-};
-
 int sm_count()
 {
     static int counts[64];
@@ -336,15 +372,68 @@ int sm_count()
     return n;
 }
 
-// The kernel's shared memory limit, set once per device.
+template <typename T, int THREADS, int HELD, int R>
+void launch_quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t qs, float *scales, cudaStream_t s)
+{
+    constexpr int PER_BLOCK = (THREADS < 256 ? 256 / THREADS : 1) * R;
+    const unsigned g = grid_x((rows + PER_BLOCK - 1) / PER_BLOCK), b = THREADS < 256 ? 256 : THREADS;
+    if (aligned(x, xs * (int64_t)sizeof(T), 16) && aligned(q, qs, Vec<T>::N))
+        k_quantize<T, THREADS, HELD, R, true><<<g, b, 0, s>>>(x, rows, cols, xs, q, qs, scales);
+    else
+        k_quantize<T, THREADS, HELD, R, false><<<g, b, 0, s>>>(x, rows, cols, xs, q, qs, scales);
+}
+
+template <typename T>
+void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t qs, float *scales, cudaStream_t s)
+{
+    const int vecs = (cols + Vec<T>::N - 1) / Vec<T>::N;
+    // few rows: one vector a thread, so that a row's latency is one load's
+    const bool few = rows <= 2 * sm_count();
+    if (vecs <= 32) launch_quantize<T, 32, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 64 && !few) launch_quantize<T, 32, 2, 2>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 128 && !few) launch_quantize<T, 32, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 128) launch_quantize<T, 128, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 512 && !few) launch_quantize<T, 128, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 1024 && few) launch_quantize<T, 1024, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 1024) launch_quantize<T, 256, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 4096) launch_quantize<T, 1024, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else k_quantize_long<T><<<grid_x(rows), 1024, 0, s>>>(x, cols, xs, q, qs, scales);
+    SC_LAUNCH_CHECK();
+    count_launch();
+}
+
+template <typename T>
+void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, int64_t rows, int cols, T *y, int64_t ys,
+                cudaStream_t s)
+{
+    constexpr int N = Vec<T>::N;
+    int log_lanes = 0;
+    while (log_lanes < 8 && (N << log_lanes) < cols) ++log_lanes;
+    const int64_t deep = (256 >> log_lanes) * 4, wide = (int64_t)N << log_lanes;
+    const dim3 g(grid_x((rows + deep - 1) / deep), (unsigned)std::min<int64_t>((cols + wide - 1) / wide, 65535));
+    if (aligned(q, qs, N) && aligned(y, ys * (int64_t)sizeof(T), 16))
+        k_dequantize<T, true><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys, log_lanes);
+    else
+        k_dequantize<T, false><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys, log_lanes);
+    SC_LAUNCH_CHECK();
+    count_launch();
+}
+
+struct Rows8 {
+    const int8_t *p;
+    int64_t stride;
+};
+
+// The kernel's shared memory limit (and clusters of 16), set once per device.
 template <typename F>
-void allow_smem(F *kernel, int bytes, std::atomic<uint64_t> &done)
+void allow_smem(F *kernel, int bytes, std::atomic<uint64_t> &done, bool wide_cluster = false)
 {
     int dev = 0;
     SC_CUDA(cudaGetDevice(&dev));
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
     SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (wide_cluster) SC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     done.fetch_or(bit, std::memory_order_relaxed);
 }
 
@@ -421,10 +510,61 @@ void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y
     count_launch();
 }
 
+// How a call with few rows runs on k_token: tokens per CTA and channels' distribution, or per_cta = 0 where
+// it does not.
+struct TokenPlan {
+    int mt, per_cta, log_s, ctas;
+};
+
+TokenPlan token_plan(int64_t rows, int64_t n, int64_t k, bool rows_out)
+{
+    TokenPlan t{rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8, 0, 0, 0};
+    if (rows > 8 || (rows_out && n > 1024)) return t;
+    const int target = rows_out ? TK_CLUSTER : 2 * sm_count();
+    // a warp for each channel, or several, down to one 512-byte step of K each, while warps are few
+    while (t.log_s < 3 && (n << t.log_s) < target * 4 && (512 << t.log_s) < k) ++t.log_s;
+    const int abreast = TK_WARPS >> t.log_s;
+    const int64_t per = ((n + target - 1) / target + abreast - 1) / abreast * abreast;
+    if (per > 4096 || token_smem(t.mt, (int)k, (int)per, t.log_s, rows_out) > 200 * 1024) return t;
+    t.per_cta = (int)per;
+    t.ctas = (int)((n + per - 1) / per);
+    return t;
+}
+
+template <typename X, int MT, bool ROWS_OUT>
+void launch_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
+{
+    static std::atomic<uint64_t> ready{0};
+    allow_smem(k_token<X, MT, ROWS_OUT>, 200 * 1024, ready, ROWS_OUT);
+    cudaLaunchAttribute attr{};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)t.ctas, (unsigned)((a.rows + MT - 1) / MT));
+    cfg.blockDim = dim3(TK_THREADS);
+    cfg.dynamicSmemBytes = (size_t)token_smem(MT, a.k, t.per_cta, t.log_s, ROWS_OUT);
+    cfg.stream = s;
+    if (ROWS_OUT) {
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = (unsigned)t.ctas;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+    }
+    SC_CUDA(cudaLaunchKernelEx(&cfg, k_token<X, MT, ROWS_OUT>, a));
+    count_launch();
+}
+
+template <typename X, bool ROWS_OUT>
+void product_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
+{
+    if (t.mt == 1) launch_token<X, 1, ROWS_OUT>(a, t, s);
+    else if (t.mt == 2) launch_token<X, 2, ROWS_OUT>(a, t, s);
+    else if (t.mt == 4) launch_token<X, 4, ROWS_OUT>(a, t, s);
+    else launch_token<X, 8, ROWS_OUT>(a, t, s);
+}
+
 // Whether the pair kernel's units leave SM pairs without work.
 bool few(int64_t rows, int64_t n) { return (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN) < 64; }
 
-int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 }  // namespace
 
@@ -444,18 +584,41 @@ void dequantize_tokens(const int8_t *q, int64_t q_stride, const float *scales, f
     else dequantize(q, q_stride, scales, scale, rows, (int)cols, (__nv_bfloat16 *)y, y_stride, s);
 }
 
-// Workspace: the rows of a float x held in 8 bits and their scales, x and w spread where TMA cannot read
-// them, and the product's rows in 32 bits where they come back quantised by a launch of their own.
-static bool own_requant(const Int8Linear &p)
+static int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+// What a call consists of.  Its workspace holds, in this order and where they are there: the scales and the
+// rows of a float x held in 8 bits, x and w spread where TMA cannot read them, and the product's rows
+// in 32 bits where a launch of their own quantises them.
+struct Plan {
+    bool token, quantise, spread_x, spread_w, requant;
+    TokenPlan t;
+    int64_t bytes;
+};
+
+static Plan plan(const Int8Linear &p)
 {
-    return p.y_type == SC_TYPE_I8 && p.y_scales && (p.n > 2 * PN || few(p.rows, p.n));
+    Plan o{};
+    const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
+    o.t = token_plan(p.rows, p.n, p.k, rows_out);
+    o.token = o.t.per_cta > 0;
+    o.quantise = p.x_type != SC_TYPE_I8 && (!o.token || rows_out);
+    o.spread_x = p.x_type == SC_TYPE_I8 && !o.token && !p.x_packed;
+    o.spread_w = !p.w_packed;
+    o.requant = rows_out && !o.token && (p.n > 2 * PN || few(p.rows, p.n));
+    if (o.quantise) o.bytes += pad(p.rows * 4, 256);
+    if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
+    if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
+    if (o.requant) o.bytes += pad(p.rows * p.n * 4, 256);
+    return o;
 }
 
+int64_t int8_linear_workspace(const Int8Linear &p) { return plan(p).bytes; }
+
+// The product without quantising its rows, on the kernel that its sizes call for.
 static void product(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride,
                     cudaStream_t s)
 {
-    const bool rows = y_type == SC_TYPE_I8 && p.y_scales;
-    if (!rows && few(p.rows, p.n)) {
+    if (few(p.rows, p.n)) {
         const int64_t nkb = (p.k + PK - 1) / PK;
         const int bt = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
         const int64_t tiles = (p.rows + bt - 1) / bt * ((p.n + 127) / 128);
@@ -464,25 +627,15 @@ static void product(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void
         if (bt == 16) product_few<16>(p, x, xs, w, y, y_type, y_stride, split, s);
         else if (bt == 32) product_few<32>(p, x, xs, w, y, y_type, y_stride, split, s);
         else product_few<64>(p, x, xs, w, y, y_type, y_stride, split, s);
-    } else if (rows) product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, y_stride, s);
-    else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, y_stride, s);
+    } else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, y_stride, s);
     else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, y_stride, s);
     else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, y_stride, s);
     else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, s);
 }
 
-int64_t int8_linear_workspace(const Int8Linear &p)
-{
-    int64_t b = 0;
-    if (p.x_type != SC_TYPE_I8) b += pad(p.rows * 4, 256);
-    if (p.x_type != SC_TYPE_I8 || !p.x_packed) b += pad(p.rows * pad(p.k, 16), 256);
-    if (!p.w_packed) b += pad(p.n * pad(p.k, 16), 256);
-    if (own_requant(p)) b += pad(p.rows * p.n * 4, 256);
-    return b;
-}
-
 void int8_linear(const Int8Linear &p, cudaStream_t s)
 {
+    const Plan o = plan(p);
     uint8_t *ws = (uint8_t *)p.workspace;
     auto take = [&](int64_t bytes) {
         uint8_t *at = ws;
@@ -498,20 +651,32 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
     };
     Rows8 x{(const int8_t *)p.x, p.x_stride}, w{p.w, p.w_stride};
     const float *xs = p.x_scales;
-    if (p.x_type != SC_TYPE_I8) {
+    const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
+    if (o.quantise) {
         float *sc = (float *)take(p.rows * 4);
         int8_t *q = (int8_t *)take(p.rows * pad(p.k, 16));
         quantize_tokens(p.x, p.x_type, p.rows, p.k, p.x_stride, q, pad(p.k, 16), sc, s);
         x = {q, pad(p.k, 16)};
         xs = sc;
-    } else if (!p.x_packed) {
+    } else if (o.spread_x) {
         x = spread(x.p, p.rows, x.stride);
     }
-    if (!p.w_packed) w = spread(p.w, p.n, p.w_stride);
-    if (own_requant(p)) {
+    if (o.spread_w) w = spread(p.w, p.n, p.w_stride);
+    if (o.token) {
+        const TokenParams a{o.quantise ? x.p : p.x, x.stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n,
+                            (int)p.k, p.relu, p.y_type, p.y, p.y_stride, p.output_scale, p.y_scales, o.t.per_cta,
+                            o.t.log_s};
+        if (rows_out) product_token<int8_t, true>(a, o.t, s);
+        else if (p.x_type == SC_TYPE_I8) product_token<int8_t, false>(a, o.t, s);
+        else if (p.x_type == SC_TYPE_F32) product_token<float, false>(a, o.t, s);
+        else if (p.x_type == SC_TYPE_F16) product_token<__half, false>(a, o.t, s);
+        else product_token<__nv_bfloat16, false>(a, o.t, s);
+    } else if (o.requant) {
         float *y = (float *)take(p.rows * p.n * 4);
         product(p, x, xs, w, y, SC_TYPE_F32, p.n, s);
         quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+    } else if (rows_out) {
+        product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)p.y, p.y_stride, s);
     } else {
         product(p, x, xs, w, p.y, p.y_type, p.y_stride, s);
     }
