@@ -24,6 +24,13 @@
 namespace sc {
 namespace {
 
+// ---- launches that overlap the end of the one before ------------------------------------------
+// Every kernel here is launched so that it may start while the kernel before it in the stream ends.  All
+// its threads wait for that kernel's results before they touch global memory, so the set-up alone
+// overlaps, and no kernel ends before the one before it has.
+__device__ __forceinline__ void previous_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- element types ---------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
@@ -140,6 +147,8 @@ k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, in
     __shared__ uint32_t tops[R][32];
     const int t = threadIdx.x % THREADS, grp = threadIdx.x / THREADS;
     const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + grp) * R;
+    next_may_start();
+    previous_done();
     uint4 v[R][HELD];
     uint32_t top[R];
 #pragma unroll
@@ -197,6 +206,8 @@ k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__r
 {
     __shared__ uint32_t tops[32];
     const T *xr = x + (int64_t)blockIdx.x * x_stride;
+    next_may_start();
+    previous_done();
     uint32_t top = 0;
     for (int64_t c = threadIdx.x; c < cols; c += 1024) top = max(top, magnitude(to_f32<T>(xr[c])));
     top = __reduce_max_sync(0xffffffffu, top);
@@ -222,6 +233,8 @@ k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__rest
     const int deep = 256 >> log_lanes;                             // rows of one pass
     const int64_t row0 = (int64_t)blockIdx.x * deep * U + (threadIdx.x >> log_lanes);
     const int lane = threadIdx.x & ((1 << log_lanes) - 1);
+    next_may_start();
+    previous_done();
     for (int64_t c64 = ((int64_t)blockIdx.y << log_lanes) * N; c64 < cols; c64 += ((int64_t)gridDim.y << log_lanes) * N) {
         const int c = (int)c64 + lane * N;
         if (c >= cols) break;
@@ -338,6 +351,8 @@ __global__ void __launch_bounds__(256)
 k_spread(const int8_t *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ y, int64_t y_stride)
 {
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    next_may_start();
+    previous_done();
     if (row >= rows) return;
     const int8_t *xr = x + row * x_stride;
     for (int c = (threadIdx.x & 31) * 4; c < cols; c += 128) {
@@ -360,6 +375,26 @@ unsigned grid_x(int64_t blocks)
     return (unsigned)blocks;
 }
 
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, unsigned cluster, A... args)
+{
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    SC_CUDA(cudaLaunchKernelEx(&cfg, kernel, (P)args...));
+    count_launch();
+}
+
 int sm_count()
 {
     static int counts[64];
@@ -378,9 +413,9 @@ void launch_quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, 
     constexpr int PER_BLOCK = (THREADS < 256 ? 256 / THREADS : 1) * R;
     const unsigned g = grid_x((rows + PER_BLOCK - 1) / PER_BLOCK), b = THREADS < 256 ? 256 : THREADS;
     if (aligned(x, xs * (int64_t)sizeof(T), 16) && aligned(q, qs, Vec<T>::N))
-        k_quantize<T, THREADS, HELD, R, true><<<g, b, 0, s>>>(x, rows, cols, xs, q, qs, scales);
+        launch(k_quantize<T, THREADS, HELD, R, true>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales);
     else
-        k_quantize<T, THREADS, HELD, R, false><<<g, b, 0, s>>>(x, rows, cols, xs, q, qs, scales);
+        launch(k_quantize<T, THREADS, HELD, R, false>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales);
 }
 
 template <typename T>
@@ -397,9 +432,7 @@ void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t
     else if (vecs <= 1024 && few) launch_quantize<T, 1024, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024) launch_quantize<T, 256, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 4096) launch_quantize<T, 1024, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
-    else k_quantize_long<T><<<grid_x(rows), 1024, 0, s>>>(x, cols, xs, q, qs, scales);
-    SC_LAUNCH_CHECK();
-    count_launch();
+    else launch(k_quantize_long<T>, grid_x(rows), 1024, 0, s, 1, x, cols, xs, q, qs, scales);
 }
 
 template <typename T>
@@ -412,11 +445,9 @@ void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, i
     const int64_t deep = (256 >> log_lanes) * 4, wide = (int64_t)N << log_lanes;
     const dim3 g(grid_x((rows + deep - 1) / deep), (unsigned)std::min<int64_t>((cols + wide - 1) / wide, 65535));
     if (aligned(q, qs, N) && aligned(y, ys * (int64_t)sizeof(T), 16))
-        k_dequantize<T, true><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys, log_lanes);
+        launch(k_dequantize<T, true>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes);
     else
-        k_dequantize<T, false><<<g, 256, 0, s>>>(q, qs, scales, scale, rows, cols, y, ys, log_lanes);
-    SC_LAUNCH_CHECK();
-    count_launch();
+        launch(k_dequantize<T, false>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes);
 }
 
 struct Rows8 {
@@ -468,19 +499,16 @@ void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y,
     const int64_t tiles = (p.rows + 2 * PM - 1) / (2 * PM), units = (p.n + PN - 1) / PN;
     const int64_t work = MODE == ROWS ? tiles : tiles * units;
     const unsigned pairs = (unsigned)std::min<int64_t>(work, sm_count() / 2);
-    k_pair<T, MODE><<<2 * pairs, P_THREADS, P_SMEM, s>>>(a);
-    SC_LAUNCH_CHECK();
-    count_launch();
+    launch(k_pair<T, MODE>, 2 * pairs, P_THREADS, P_SMEM, s, 2, a);
 }
 
 // y (float types, or int8 by one scale) of few int8 rows; `bt` tokens per tile, K split over `split` CTAs
-template <int BT>
-void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride, int split,
-                 cudaStream_t s)
+template <int BT, typename T>
+void launch_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, int split, cudaStream_t s)
 {
     using C = FewCfg<BT>;
     static std::atomic<uint64_t> ready{0};
-    allow_smem(k_few<BT>, C::SMEM, ready);
+    allow_smem(k_few<BT, T>, C::SMEM, ready);
     FewParams a;
     a.w = tensor_map(w.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.n, w.stride, PK, 128);
     a.x = tensor_map(x.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.rows, x.stride, PK, BT);
@@ -491,80 +519,90 @@ void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y
     a.n = (int)p.n;
     a.k = (int)p.k;
     a.relu = p.relu;
-    a.y_type = y_type;
     a.y = y;
     a.y_stride = y_stride;
+    a.y_vec = aligned(y, y_stride * (int64_t)sizeof(T), 4 * sizeof(T));
     a.output_scale = p.output_scale;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)split;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)split, (unsigned)((p.n + 127) / 128), (unsigned)((p.rows + BT - 1) / BT));
-    cfg.blockDim = dim3(F_THREADS);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    SC_CUDA(cudaLaunchKernelEx(&cfg, k_few<BT>, a));
-    count_launch();
+    launch(k_few<BT, T>, dim3((unsigned)split, (unsigned)((p.n + 127) / 128), (unsigned)((p.rows + BT - 1) / BT)), F_THREADS,
+           C::SMEM, s, (unsigned)split, a);
 }
 
-// How a call with few rows runs on k_token: tokens per CTA and channels' distribution, or per_cta = 0 where
-// it does not.
+template <int BT>
+void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride, int split,
+                 cudaStream_t s)
+{
+    if (y_type == SC_TYPE_F32) launch_few<BT>(p, x, xs, w, (float *)y, y_stride, split, s);
+    else if (y_type == SC_TYPE_F16) launch_few<BT>(p, x, xs, w, (__half *)y, y_stride, split, s);
+    else if (y_type == SC_TYPE_BF16) launch_few<BT>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, split, s);
+    else launch_few<BT>(p, x, xs, w, (int8_t *)y, y_stride, split, s);
+}
+
+// How one or two rows run on k_token; per_cta = 0 where they do not.
 struct TokenPlan {
-    int mt, per_cta, log_s, ctas;
+    int per_cta, log_s, ctas;
 };
 
-TokenPlan token_plan(int64_t rows, int64_t n, int64_t k, bool rows_out)
+TokenPlan token_plan(int64_t rows, int64_t n, int64_t k)
 {
-    TokenPlan t{rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8, 0, 0, 0};
-    if (rows > 8 || (rows_out && n > 1024)) return t;
-    const int target = rows_out ? TK_CLUSTER : 2 * sm_count();
-    // a warp for each channel, or several, down to one 512-byte step of K each, while warps are few
-    while (t.log_s < 3 && (n << t.log_s) < target * 4 && (512 << t.log_s) < k) ++t.log_s;
-    const int abreast = TK_WARPS >> t.log_s;
+    TokenPlan t{0, 0, 0};
+    if (rows > 2) return t;
+    const int target = 2 * sm_count();
+    // a warp for four channels, or several, down to one 512-byte step of K each, while warps are few
+    while (t.log_s < 3 && (n << t.log_s) < (int64_t)target * TK_WARPS * TK_CH && (512 << t.log_s) < k) ++t.log_s;
+    const int abreast = (TK_WARPS >> t.log_s) * TK_CH;
     const int64_t per = ((n + target - 1) / target + abreast - 1) / abreast * abreast;
-    if (per > 4096 || token_smem(t.mt, (int)k, (int)per, t.log_s, rows_out) > 200 * 1024) return t;
+    // two CTAs to an SM
+    if (per > 4096 || token_smem((int)rows, (int)k, (int)per, t.log_s) > TK_SMEM) return t;
     t.per_cta = (int)per;
     t.ctas = (int)((n + per - 1) / per);
     return t;
 }
 
-template <typename X, int MT, bool ROWS_OUT>
+template <typename X, int MT>
 void launch_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
 {
     static std::atomic<uint64_t> ready{0};
-    allow_smem(k_token<X, MT, ROWS_OUT>, 200 * 1024, ready, ROWS_OUT);
-    cudaLaunchAttribute attr{};
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)t.ctas, (unsigned)((a.rows + MT - 1) / MT));
-    cfg.blockDim = dim3(TK_THREADS);
-    cfg.dynamicSmemBytes = (size_t)token_smem(MT, a.k, t.per_cta, t.log_s, ROWS_OUT);
-    cfg.stream = s;
-    if (ROWS_OUT) {
-        attr.id = cudaLaunchAttributeClusterDimension;
-        attr.val.clusterDim.x = (unsigned)t.ctas;
-        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-        cfg.attrs = &attr;
-        cfg.numAttrs = 1;
-    }
-    SC_CUDA(cudaLaunchKernelEx(&cfg, k_token<X, MT, ROWS_OUT>, a));
-    count_launch();
+    allow_smem(k_token<X, MT>, TK_SMEM, ready);
+    launch(k_token<X, MT>, (unsigned)t.ctas, TK_THREADS, (size_t)token_smem(MT, a.k, t.per_cta, t.log_s), s, 1, a);
 }
 
-template <typename X, bool ROWS_OUT>
+template <typename X>
 void product_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
 {
-    if (t.mt == 1) launch_token<X, 1, ROWS_OUT>(a, t, s);
-    else if (t.mt == 2) launch_token<X, 2, ROWS_OUT>(a, t, s);
-    else if (t.mt == 4) launch_token<X, 4, ROWS_OUT>(a, t, s);
-    else launch_token<X, 8, ROWS_OUT>(a, t, s);
+    if (a.rows == 1) launch_token<X, 1>(a, t, s);
+    else launch_token<X, 2>(a, t, s);
 }
 
-// Whether the pair kernel's units leave SM pairs without work.
-bool few(int64_t rows, int64_t n) { return (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN) < 64; }
+// Which kernel multiplies more than two rows, from the time in microseconds that each is expected to take:
+// so many waves of CTAs, each of them a start and an end plus its K blocks.  Fitted to measurements at 1 to
+// 3,000 rows of seven layers (512 x 512 to 8,192 x 2,048); among them, k_few against k_pair:
+//   K = 512, N = 512:     16 rows 3.4 / 5.9,  1,000 rows 4.5 / 6.5,  3,000 rows 7.9 / 6.6
+//   K = 8,192, N = 512:   16 rows 4.9 / 22,  1,000 rows 11.9 / 23,  3,000 rows 24.1 / 23.4
+//   K = 4,096, N = 4,096: 16 rows 5.9 / 13.8,  400 rows 15.8 / 14.8,  1,000 rows 29.9 / 15.8
+struct MatrixPlan {
+    int bt, split;               // k_few's tile and split of K, or bt = 0: k_pair
+};
 
+MatrixPlan matrix_plan(int64_t rows, int64_t n, int64_t k)
+{
+    const int64_t nkb = (k + PK - 1) / PK, sms = sm_count();
+    const int64_t units = (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN);
+    MatrixPlan best{0, 1};
+    double least = 5.0 + (double)((units + sms / 2 - 1) / (sms / 2)) * (0.3 * (double)nkb + 0.9);
+    const struct { int bt; double fixed, block; } tiles[] = {{16, 2.9, 0.24}, {32, 3.4, 0.25}, {64, 4.3, 0.27}, {128, 6.1, 0.33}};
+    for (const auto &t : tiles) {
+        const int64_t count = (rows + t.bt - 1) / t.bt * ((n + 127) / 128);
+        if (count > 4 * sms || (t.bt > 16 && rows <= t.bt / 2)) continue;
+        int split = 1;
+        while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * count <= sms) split *= 2;
+        const double time = (double)((count * split + sms - 1) / sms) * (t.fixed + t.block * (double)((nkb + split - 1) / split));
+        if (time < least) {
+            least = time;
+            best = {t.bt, split};
+        }
+    }
+    return best;
+}
 
 }  // namespace
 
@@ -590,8 +628,9 @@ static int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 // rows of a float x held in 8 bits, x and w spread where TMA cannot read them, and the product's rows
 // in 32 bits where a launch of their own quantises them.
 struct Plan {
-    bool token, quantise, spread_x, spread_w, requant;
+    bool quantise, spread_x, spread_w, requant;
     TokenPlan t;
+    MatrixPlan m;
     int64_t bytes;
 };
 
@@ -599,12 +638,13 @@ static Plan plan(const Int8Linear &p)
 {
     Plan o{};
     const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
-    o.t = token_plan(p.rows, p.n, p.k, rows_out);
-    o.token = o.t.per_cta > 0;
-    o.quantise = p.x_type != SC_TYPE_I8 && (!o.token || rows_out);
-    o.spread_x = p.x_type == SC_TYPE_I8 && !o.token && !p.x_packed;
+    o.t = token_plan(p.rows, p.n, p.k);
+    const bool token = o.t.per_cta > 0;
+    if (!token) o.m = matrix_plan(p.rows, p.n, p.k);
+    o.quantise = p.x_type != SC_TYPE_I8 && !token;
+    o.spread_x = p.x_type == SC_TYPE_I8 && !token && !p.x_packed;
     o.spread_w = !p.w_packed;
-    o.requant = rows_out && !o.token && (p.n > 2 * PN || few(p.rows, p.n));
+    o.requant = rows_out && (token || o.m.bt > 0 || p.n > 2 * PN);
     if (o.quantise) o.bytes += pad(p.rows * 4, 256);
     if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
     if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
@@ -613,25 +653,6 @@ static Plan plan(const Int8Linear &p)
 }
 
 int64_t int8_linear_workspace(const Int8Linear &p) { return plan(p).bytes; }
-
-// The product without quantising its rows, on the kernel that its sizes call for.
-static void product(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride,
-                    cudaStream_t s)
-{
-    if (few(p.rows, p.n)) {
-        const int64_t nkb = (p.k + PK - 1) / PK;
-        const int bt = p.rows <= 16 ? 16 : p.rows <= 32 ? 32 : 64;
-        const int64_t tiles = (p.rows + bt - 1) / bt * ((p.n + 127) / 128);
-        int split = 1;
-        while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * tiles <= sm_count()) split *= 2;
-        if (bt == 16) product_few<16>(p, x, xs, w, y, y_type, y_stride, split, s);
-        else if (bt == 32) product_few<32>(p, x, xs, w, y, y_type, y_stride, split, s);
-        else product_few<64>(p, x, xs, w, y, y_type, y_stride, split, s);
-    } else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, y_stride, s);
-    else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, y_stride, s);
-    else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, y_stride, s);
-    else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, s);
-}
 
 void int8_linear(const Int8Linear &p, cudaStream_t s)
 {
@@ -644,14 +665,11 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
     };
     auto spread = [&](const int8_t *from, int64_t rows, int64_t stride) {
         int8_t *to = (int8_t *)take(rows * pad(p.k, 16));
-        k_spread<<<grid_x((rows + 7) / 8), 256, 0, s>>>(from, rows, (int)p.k, stride, to, pad(p.k, 16));
-        SC_LAUNCH_CHECK();
-        count_launch();
+        launch(k_spread, grid_x((rows + 7) / 8), 256, 0, s, 1, from, rows, p.k, stride, to, pad(p.k, 16));
         return Rows8{to, pad(p.k, 16)};
     };
     Rows8 x{(const int8_t *)p.x, p.x_stride}, w{p.w, p.w_stride};
     const float *xs = p.x_scales;
-    const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
     if (o.quantise) {
         float *sc = (float *)take(p.rows * 4);
         int8_t *q = (int8_t *)take(p.rows * pad(p.k, 16));
@@ -662,24 +680,27 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
         x = spread(x.p, p.rows, x.stride);
     }
     if (o.spread_w) w = spread(p.w, p.n, p.w_stride);
-    if (o.token) {
-        const TokenParams a{o.quantise ? x.p : p.x, x.stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n,
-                            (int)p.k, p.relu, p.y_type, p.y, p.y_stride, p.output_scale, p.y_scales, o.t.per_cta,
-                            o.t.log_s};
-        if (rows_out) product_token<int8_t, true>(a, o.t, s);
-        else if (p.x_type == SC_TYPE_I8) product_token<int8_t, false>(a, o.t, s);
-        else if (p.x_type == SC_TYPE_F32) product_token<float, false>(a, o.t, s);
-        else if (p.x_type == SC_TYPE_F16) product_token<__half, false>(a, o.t, s);
-        else product_token<__nv_bfloat16, false>(a, o.t, s);
-    } else if (o.requant) {
-        float *y = (float *)take(p.rows * p.n * 4);
-        product(p, x, xs, w, y, SC_TYPE_F32, p.n, s);
-        quantize(y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
-    } else if (rows_out) {
-        product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)p.y, p.y_stride, s);
-    } else {
-        product(p, x, xs, w, p.y, p.y_type, p.y_stride, s);
-    }
+    // the product itself: to y, or in 32 bits to the workspace
+    void *y = o.requant ? take(p.rows * p.n * 4) : p.y;
+    const int y_type = o.requant ? SC_TYPE_F32 : p.y_type;
+    const int64_t ys = o.requant ? p.n : p.y_stride;
+    if (o.t.per_cta > 0) {
+        const TokenParams a{p.x, p.x_stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k, p.relu,
+                            y_type, y, ys, p.output_scale, o.t.per_cta, o.t.log_s};
+        if (p.x_type == SC_TYPE_I8) product_token<int8_t>(a, o.t, s);
+        else if (p.x_type == SC_TYPE_F32) product_token<float>(a, o.t, s);
+        else if (p.x_type == SC_TYPE_F16) product_token<__half>(a, o.t, s);
+        else product_token<__nv_bfloat16>(a, o.t, s);
+    } else if (o.m.bt == 16) product_few<16>(p, x, xs, w, y, y_type, ys, o.m.split, s);
+    else if (o.m.bt == 32) product_few<32>(p, x, xs, w, y, y_type, ys, o.m.split, s);
+    else if (o.m.bt == 64) product_few<64>(p, x, xs, w, y, y_type, ys, o.m.split, s);
+    else if (o.m.bt == 128) product_few<128>(p, x, xs, w, y, y_type, ys, o.m.split, s);
+    else if (y_type == SC_TYPE_I8 && p.y_scales) product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, ys, s);
+    else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, ys, s);
+    else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, ys, s);
+    else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, ys, s);
+    else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, ys, s);
+    if (o.requant) quantize((const float *)y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
 }
 
 int int8_device_error()

@@ -61,6 +61,16 @@ struct PairParams {
     float output_scale;
 };
 
+// One lane of a converged warp, the same each time.  The loops around TMA and MMA are run by whole warps
+// and only the instructions themselves by this lane: under a branch on the lane's number the compiler
+// has to take their operands through a loop over the lanes, which costs over 100 clocks each.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void tma_store_2d(const void *tmap, const void *smem, int32_t x, int32_t y)
 {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
@@ -81,6 +91,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+
+// shared memory of this CTA -> shared memory of another one of the cluster, signalled on its barrier
+__device__ __forceinline__ void bulk_copy_to(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "r"(smem_u32(src)), "r"(bytes), "r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -121,13 +138,14 @@ __device__ __forceinline__ void store_tile(const PairParams &p, const uint8_t *t
     if (p.y_tma) {
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0 && row0 < p.rows && col0 < p.n) {
+        if (row0 < p.rows && col0 < p.n && elect_one()) {
             tma_store_2d(&p.y, tile, col0, (int32_t)row0);
             bulk_commit();
         }
     } else {
         __syncwarp();
         const int nr = (int)min((int64_t)32, p.rows - row0);
+#pragma unroll 4
         for (int r = 0; r < nr; ++r)
 #pragma unroll
             for (int c = lane; c < COLS; c += 32) {
@@ -143,12 +161,12 @@ __device__ __forceinline__ void store_tile(const PairParams &p, const uint8_t *t
 // the staging tile may be written again
 __device__ __forceinline__ void staging_free(const PairParams &p, int lane)
 {
-    if (p.y_tma && lane == 0) bulk_wait_read();
+    if (p.y_tma && elect_one()) bulk_wait_read();
     __syncwarp();
 }
 
 template <typename T, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ PairParams p)
+__global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ PairParams p)
 {
     constexpr bool REQUANT = MODE == ROWS;
     extern __shared__ uint8_t smem_raw[];
@@ -190,59 +208,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair
     __syncthreads();
     cluster_sync();                                            // both CTAs' barriers exist
     tc_fence_after();
+    next_may_start();
+    previous_done();
     const uint32_t tmem_base = *tmem_slot;
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int64_t g = pair * group; g < units && ok; g += pairs * group)
-                for (int64_t u = g; u < g + group && ok; ++u) {
-                    const int row0 = (int)(u / nu) * 2 * PM + (int)rank * PM;
-                    const int col0 = (int)(u % nu) * PN + (int)rank * (PN / 2);
-                    for (int kb = 0; kb < nkb; ++kb, ++it) {
-                        const int s = it % P_STAGES;
-                        if (!(ok = mbar_wait_cluster(&empty[s], ((it / P_STAGES) & 1) ^ 1))) break;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t g = pair * group; g < units && ok; g += pairs * group)
+            for (int64_t u = g; u < g + group && ok; ++u) {
+                const int row0 = (int)(u / nu) * 2 * PM + (int)rank * PM;
+                const int col0 = (int)(u % nu) * PN + (int)rank * (PN / 2);
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const int s = it % P_STAGES;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty[s], ((it / P_STAGES) & 1) ^ 1)))) break;
+                    if (elect_one()) {
                         uint8_t *st = smem + s * P_STAGE;
                         const uint32_t fb = map_to_rank(&full[s], 0);
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * P_STAGE);
                         tma_load_2d_pair(st, &p.x, fb, kb * PK, row0);
                         tma_load_2d_pair(st + P_A, &p.w, fb, kb * PK, col0);
                     }
+                    __syncwarp();
                 }
-            if (!ok) {
-                // gave up: loads issued into this CTA may still land, see the fused kernels' abort path
-                for (uint32_t i = it > (uint32_t)P_STAGES ? it - P_STAGES : 0; i < it; ++i)
-                    mbar_wait_cluster_drain(rank == 0 ? &full[i % P_STAGES] : &empty[i % P_STAGES], (i / P_STAGES) & 1);
-                spin_ns(100000);
             }
+        if (!ok) {
+            // gave up: loads issued into this CTA may still land, see the fused kernels' abort path
+            for (uint32_t i = it > (uint32_t)P_STAGES ? it - P_STAGES : 0; i < it; ++i)
+                mbar_wait_cluster_drain(rank == 0 ? &full[i % P_STAGES] : &empty[i % P_STAGES], (i / P_STAGES) & 1);
+            spin_ns(100000);
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr uint32_t idesc = idesc_i8(2 * PM, PN);
             uint32_t it = 0, uu = 0;
             bool ok = true;
             for (int64_t g = pair * group; g < units && ok; g += pairs * group)
                 for (int64_t u = g; u < g + group && ok; ++u, ++uu) {
                     const int ab = uu & 1;
-                    if (!(ok = mbar_wait_cluster(&acc_empty[ab], ((uu >> 1) & 1) ^ 1))) break;
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[ab], ((uu >> 1) & 1) ^ 1)))) break;
                     tc_fence_after();
                     const uint32_t d = tmem_base + ab * PN;
                     for (int kb = 0; kb < nkb; ++kb, ++it) {
                         const int s = it % P_STAGES;
-                        if (!(ok = mbar_wait_cluster(&full[s], (it / P_STAGES) & 1))) break;
+                        if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[s], (it / P_STAGES) & 1)))) break;
                         tc_fence_after();
-                        const uint32_t a = smem_u32(smem + s * P_STAGE), b = a + P_A;
-                        const int steps = kb == nkb - 1 ? last_k32 : PK / 32;
-                        for (int i = 0; i < steps; ++i)
-                            mma_i8_pair(d, smem_desc_sw128(a + 32 * i), smem_desc_sw128(b + 32 * i), idesc,
-                                        (kb | i) ? 1u : 0u);
-                        mma_commit_pair(&empty[s], 0x3);
+                        if (elect_one()) {
+                            const uint64_t a = smem_desc_sw128(smem_u32(smem + s * P_STAGE));
+                            const uint64_t b = smem_desc_sw128(smem_u32(smem + s * P_STAGE + P_A));
+                            const int steps = kb == nkb - 1 ? last_k32 : PK / 32;
+#pragma unroll
+                            for (int i = 0; i < PK / 32; ++i)          // 32 bytes further: 2 in the descriptor's units
+                                if (i < steps) mma_i8_pair(d, a + 2 * i, b + 2 * i, idesc, (kb | i) ? 1u : 0u);
+                            mma_commit_pair(&empty[s], 0x3);
+                            if (kb == nkb - 1) mma_commit_pair(&acc_full[ab], 0x3);
+                        }
+                        __syncwarp();
                     }
-                    if (ok) mma_commit_pair(&acc_full[ab], 0x3);
                 }
-            mma_commit_pair(drain, 0x3);                       // completes after every MMA and commit above
+            if (elect_one()) mma_commit_pair(drain, 0x3);              // completes after every MMA and commit above
         }
         __syncwarp();
     } else {
@@ -379,7 +404,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair
                 uu += nu;
             }
         }
-        if (p.y_tma && lane == 0) bulk_wait_all();
+        if (p.y_tma && elect_one()) bulk_wait_all();
         __syncwarp();
     }
     if (warp == 1) mbar_wait_cluster_drain(drain, 0);
@@ -397,16 +422,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(P_THREADS, 1) k_pair
 // With few rows the weights are what has to be read, so they take the side of the MMA that is always
 // full: a CTA computes 128 channels (M) x BT tokens (N = 16, 32, 64 or 128), and where such tiles are fewer
 // than the SMs a cluster of up to eight CTAs splits the tile's K.  Each CTA then owns BT / S of the tokens:
-// the others put their whole sums for them into its shared memory, 128 channels at a time, one
-// cluster barrier publishes them, and the owner adds the S parts (whole numbers: any order) and writes
-// the results, neighbouring lanes writing neighbouring channels.  No workspace, no counters, one launch.
+// the others send it their whole sums for them, one bulk copy into its shared memory each, and the owner adds
+// the S parts (whole numbers: any order) and writes the results, a warp writing a token's 128 channels at
+// once.  No workspace, no counters, one launch.  (Stores to the owner's memory by each thread, and a cluster
+// barrier, took 10,500 clocks for 64 tokens.)
 //
 // Warps: 0 TMA producer, 1 MMA issuer, 2-5 epilogue (one for each TMEM lane quarter).
 struct FewParams {
     CUtensorMap w, x;                          // boxes 128 and BT rows x 128 bytes
     const float *xs, *ws, *bias;
     int64_t rows;
-    int n, k, relu, y_type;
+    int n, k, relu, y_vec;                     // y_vec: four results of y lie on a multiple of their size
     void *y;
     int64_t y_stride;
     float output_scale;
@@ -427,26 +453,36 @@ template <int BT>
 struct FewCfg {
     static constexpr int STAGES = BT <= 32 ? 9 : BT == 64 ? 7 : 4;
     static constexpr int STAGE = 128 * PK + BT * PK;
-    static constexpr int OFF_RECV = STAGES * STAGE;                    // [S][BT / S][128] sums of the owned tokens
+    static constexpr int OFF_RECV = STAGES * STAGE;                    // [S - 1][BT / S][128] sums from the other CTAs
     static constexpr int OFF_BAR = OFF_RECV + BT * 128 * 4;
-    static constexpr int OFF_TMEM = OFF_BAR + (2 * STAGES + 1) * 8;
-    static constexpr int SMEM = OFF_TMEM + 16 + 1024;
+    static constexpr int OFF_TMEM = OFF_BAR + (2 * STAGES + 2) * 8;
+    static constexpr int OFF_XS = OFF_TMEM + 16;                       // the tokens' scales
+    static constexpr int SMEM = OFF_XS + BT * 4 + 1024;
     static constexpr int TMEM = BT < 32 ? 32 : BT;
-    static_assert(SMEM <= 232448, "shared memory per CTA");
+    static_assert(SMEM <= 232448 && BT * 128 * 4 <= STAGES * STAGE, "shared memory per CTA");
 };
 
-template <int BT>
+template <typename T>
+__device__ __forceinline__ T result(float y, float output_scale)
+{
+    if constexpr (sizeof(T) == 1) return (T)static_bits(y, output_scale);
+    else return from_f32<T>(y);
+}
+
+template <int BT, typename T>
 __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ FewParams p)
 {
     using C = FewCfg<BT>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = (uint64_t *)(smem + C::OFF_BAR), *empty = full + C::STAGES, *done = empty + C::STAGES;
+    uint64_t *got = done + 1;                                          // the other CTAs' sums
     uint32_t *tmem_slot = (uint32_t *)(smem + C::OFF_TMEM);
     int32_t *recv = (int32_t *)(smem + C::OFF_RECV);
+    float *xs = (float *)(smem + C::OFF_XS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int S = gridDim.x;                                           // the cluster: x is the split
-    const int part = blockIdx.x;
+    const int S = gridDim.x;                                           // the cluster: x is the split, a power of two
+    const int part = blockIdx.x, own = BT / S;                         // at most BT / 2 parts
     const int c0 = blockIdx.y * 128;
     const int64_t t0 = (int64_t)blockIdx.z * BT;
     const int nkb_all = (p.k + PK - 1) / PK;
@@ -459,7 +495,9 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             mbar_init(&empty[s], 1);
         }
         mbar_init(done, 1);
+        mbar_init(got, 1);
         fence_mbar_init();
+        if (S > 1) mbar_arrive_expect_tx(got, (uint32_t)((S - 1) * own * 128 * 4));
         prefetch_tmap(&p.w);
         prefetch_tmap(&p.x);
     }
@@ -472,96 +510,145 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
     tc_fence_after();
     if (S > 1) cluster_arrive();                                       // this CTA runs: its memory may be written
     const uint32_t tmem = *tmem_slot;
+    next_may_start();
+    previous_done();
 
-    bool ok = true;
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % C::STAGES;
-                if (!(ok = mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1))) break;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)))) break;
+            if (elect_one()) {
                 uint8_t *st = smem + s * C::STAGE;
                 mbar_arrive_expect_tx(&full[s], C::STAGE);
                 tma_load_2d(st, &p.w, &full[s], kb * PK, c0);
                 tma_load_2d(st + 128 * PK, &p.x, &full[s], kb * PK, (int)t0);
             }
-            if (!ok) {                                                 // loads still landing, then end
-                for (uint32_t i = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; i < it; ++i)
-                    mbar_wait_cluster_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
-                spin_ns(100000);
-            }
+            __syncwarp();
+        }
+        if (!ok) {                                                     // loads still landing, then end
+            for (uint32_t i = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; i < it; ++i)
+                mbar_wait_cluster_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
+            spin_ns(100000);
         }
         __syncwarp();
         if (S > 1) cluster_wait();
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_i8(128, BT);
-            uint32_t it = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int s = it % C::STAGES;
-                if (!(ok = mbar_wait(&full[s], (it / C::STAGES) & 1))) break;
-                tc_fence_after();
-                const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + 128 * PK;
+        constexpr uint32_t idesc = idesc_i8(128, BT);
+        uint32_t it = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+            const int s = it % C::STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / C::STAGES) & 1))) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t a = smem_desc_sw128(smem_u32(smem + s * C::STAGE));
+                const uint64_t b = smem_desc_sw128(smem_u32(smem + s * C::STAGE + 128 * PK));
                 const int steps = kb == nkb_all - 1 ? last_k32 : PK / 32;
-                for (int i = 0; i < steps; ++i)
-                    mma_i8(tmem, smem_desc_sw128(a + 32 * i), smem_desc_sw128(b + 32 * i), idesc, (it | i) ? 1u : 0u);
+#pragma unroll
+                for (int i = 0; i < PK / 32; ++i)
+                    if (i < steps) mma_i8(tmem, a + 2 * i, b + 2 * i, idesc, (it | i) ? 1u : 0u);
                 mma_commit(&empty[s]);
             }
-            mma_commit(done);                                          // after every MMA above, given up or not
+            __syncwarp();
         }
+        if (elect_one()) mma_commit(done);                             // after every MMA above, given up or not
         __syncwarp();
         if (S > 1) cluster_wait();
     } else {
-        // this thread's channel; tokens are the columns
-        const int q = warp & 3, ch = c0 + q * 32 + lane;
-        const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
-        mbar_wait(done, 0);
-        __syncwarp();
-        if (S > 1) cluster_wait();
-        tc_fence_after();
+        // a channel is a lane of TMEM; tokens are the columns
+        const int q = warp & 3;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-        const int own = BT / S;                                        // S is a power of two, at most BT / 2
+        for (int i = threadIdx.x - 64; i < BT; i += 128) xs[i] = t0 + i < p.rows ? p.xs[t0 + i] : 0.0f;
+        if (S == 1) {
+            const int ch = c0 + q * 32 + lane;
+            const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
+            asm volatile("bar.sync 1, 128;" ::: "memory");             // the scales are there: warps 2-5, none has left
+            mbar_wait(done, 0);
+            __syncwarp();
+            tc_fence_after();
+            T *to = reinterpret_cast<T *>(p.y) + t0 * p.y_stride + ch;
 #pragma unroll 1
-        for (int j0 = 0; j0 < BT; j0 += 16) {
-            if (t0 + j0 >= p.rows) break;
-            uint32_t v[16];
-            tmem_ld16(taddr + j0, v);
-            tmem_ld_wait();
-            if (S == 1) {
+            for (int j0 = 0; j0 < BT && t0 + j0 < p.rows; j0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(taddr + j0, v);
+                tmem_ld_wait();
+                const int live = (int)min((int64_t)16, p.rows - t0 - j0);
+                if (ch < p.n) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int64_t r = t0 + j0 + j;
-                    if (r < p.rows && ch < p.n)
-                        store_one(p.y, p.y_type, r * p.y_stride + ch, affine((int32_t)v[j], p.xs[r], t, b, p.relu),
-                                  p.output_scale);
+                    for (int j = 0; j < 16; ++j)
+                        if (j < live)
+                            to[j * p.y_stride] = result<T>(affine((int32_t)v[j], xs[j0 + j], t, b, p.relu), p.output_scale);
                 }
-            } else {
+                to += 16 * p.y_stride;
+                __syncwarp();
+            }
+            tc_fence_before();
+        } else {
+            float t[4] = {}, b[4] = {};                                // of this lane's four channels
+            const int ch = c0 + 4 * lane;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int col = j0 + j;
-                    const uint32_t at = map_to_rank(recv + (part * own + col % own) * 128 + q * 32 + lane, col / own);
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v[j]) : "memory");
+            for (int i = 0; i < 4; ++i)
+                if (ch + i < p.n) {
+                    t[i] = p.ws[ch + i];
+                    b[i] = p.bias ? p.bias[ch + i] : 0.0f;
+                }
+            mbar_wait(done, 0);
+            __syncwarp();
+            tc_fence_after();
+            // the stages are read: their memory takes the sums, token by token
+            int32_t *sums = (int32_t *)smem + q * 32 + lane;
+#pragma unroll 1
+            for (int j0 = 0; j0 < BT; j0 += 16) {
+                uint32_t v[16];
+                tmem_ld16(taddr + j0, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sums[(j0 + j) * 128] = (int32_t)v[j];
+            }
+            tc_fence_before();
+            fence_proxy_async_smem();
+            asm volatile("bar.sync 1, 128;" ::: "memory");             // warps 2-5; none has left
+            cluster_wait();                                            // every CTA of the cluster runs
+            if (warp == 2 && elect_one()) {
+                for (int r = 1; r < S; ++r) {                          // to each owner, a different one first
+                    const int to = (part + r) & (S - 1);
+                    bulk_copy_to(map_to_rank(recv + (part < to ? part : part - 1) * own * 128, (uint32_t)to),
+                                 (int32_t *)smem + to * own * 128, (uint32_t)(own * 128 * 4), map_to_rank(got, (uint32_t)to));
+                }
+            }
+            __syncwarp();
+            mbar_wait_cluster(got, 0);
+            __syncwarp();
+#pragma unroll 2
+            for (int j = warp - 2; j < own; j += 4) {
+                const int64_t r = t0 + part * own + j;
+                int4 sum = *reinterpret_cast<const int4 *>((const int32_t *)smem + (part * own + j) * 128 + 4 * lane);
+                for (int i = 0; i < S - 1; ++i) {
+                    const int4 o = *reinterpret_cast<const int4 *>(recv + (i * own + j) * 128 + 4 * lane);
+                    sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+                }
+                if (r >= p.rows) continue;
+                const float s = xs[part * own + j];
+                T *to = reinterpret_cast<T *>(p.y) + r * p.y_stride + ch;
+                __align__(16) T o[4] = {result<T>(affine(sum.x, s, t[0], b[0], p.relu), p.output_scale),
+                                        result<T>(affine(sum.y, s, t[1], b[1], p.relu), p.output_scale),
+                                        result<T>(affine(sum.z, s, t[2], b[2], p.relu), p.output_scale),
+                                        result<T>(affine(sum.w, s, t[3], b[3], p.relu), p.output_scale)};
+                if (p.y_vec && ch + 4 <= p.n) {
+                    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(o);
+                    else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(o);
+                    else *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (ch + i < p.n) to[i] = o[i];
                 }
             }
         }
-        tc_fence_before();
     }
     __syncthreads();
-    if (S > 1) {
-        cluster_sync();                                                // every CTA's sums are where they belong
-        if (warp >= 2) {
-            const int q = warp & 3, ch = c0 + q * 32 + lane;
-            const int own = BT / S;
-            const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
-            for (int j = 0; j < own; ++j) {
-                const int64_t r = t0 + part * own + j;
-                if (r >= p.rows || ch >= p.n) break;
-                int32_t sum = 0;
-                for (int i = 0; i < S; ++i) sum += recv[(i * own + j) * 128 + q * 32 + lane];
-                store_one(p.y, p.y_type, r * p.y_stride + ch, affine(sum, p.xs[r], t, b, p.relu), p.output_scale);
-            }
-        }
-    }
+    if (S > 1) cluster_sync();                                         // what this CTA sent has been received
     if (warp == 1) {
         mbar_wait_cluster_drain(done, 0);
         tc_fence_after();

@@ -4,16 +4,14 @@
 namespace sc {
 namespace {
 
-// With one to eight rows a layer costs one reading of its weights, and no tile fills a tensor core, so
+// With one or two rows a layer costs one reading of its weights, and no tile fills a tensor core, so
 // what counts is how soon every byte of them is in flight and how little comes before and after:
-// no tensor memory, no barriers in memory, one launch.  A warp reads a channel's row (or one of S parts of
-// it, where the channels alone would leave SMs idle) in 512-byte steps and multiplies it with dp4a against
-// the tokens, which lie in shared memory; the first U steps are requested before the tokens are there.
+// no tensor memory, no barriers in memory, one launch, little code.  A warp takes four channels at a time
+// and walks their rows (or one of S parts of them, where the channels alone would leave SMs idle) in
+// 512-byte steps, two steps ahead, multiplying with dp4a against the tokens in shared memory; a token's
+// vector is read once for the four channels.  The first steps are requested before the tokens are there.
 // Float tokens are quantised on the way to shared memory by every CTA for itself, which costs a
 // reading of the token from L2 and saves a launch.
-//
-// Requantised rows (ROWS_OUT): the CTAs along x are one cluster and have all channels between them; they
-// exchange their rows' maxima through shared memory.
 struct TokenParams {
     const void *x;
     int64_t x_stride;
@@ -26,87 +24,88 @@ struct TokenParams {
     void *y;
     int64_t y_stride;
     float output_scale;
-    float *y_scales;
-    int per_cta;                     // channels of a CTA, a multiple of 8 >> log_s
+    int per_cta;                     // channels of a CTA, a multiple of 4 * (8 >> log_s)
     int log_s;                       // 2^log_s warps share a channel
 };
 
 constexpr int TK_WARPS = 8, TK_THREADS = 32 * TK_WARPS;
-constexpr int TK_CLUSTER = 16;       // CTAs that share a row's maximum, at most
+constexpr int TK_SMEM = 100 * 1024;   // two CTAs to an SM
+constexpr int TK_CH = 4;             // channels a warp takes at a time
 
-__host__ __device__ inline int token_smem(int mt, int k, int per_cta, int log_s, bool rows_out)
+__host__ __device__ inline int token_smem(int mt, int k, int per_cta, int log_s)
 {
-    return mt * ((k + 15) / 16 * 16) + mt * 4 + (per_cta << log_s) * mt * 4 +
-           (rows_out ? per_cta * mt * 4 + (TK_CLUSTER + 1) * mt * 4 : 0) + TK_WARPS * 4;
+    return mt * ((k + 15) / 16 * 16) + mt * 4 + (per_cta << log_s) * mt * 4 + TK_WARPS * 4;
 }
 
-// 16 bytes of a weight row; what lies behind its end counts as zero
-__device__ __forceinline__ uint4 weight_vec(const int8_t *row, int at, int k)
+// 16 bytes of an int8 row that ends within them; what lies behind its end counts as zero
+__device__ __noinline__ uint4 last_vec(const int8_t *row, int at, int k)
 {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (at + 16 <= k) {
-        asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-            : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + at));
-    } else {
-        int8_t *e = reinterpret_cast<int8_t *>(&v);
-        for (int i = 0; at + i < k; ++i) e[i] = row[at + i];
-    }
-    return v;
+    uint32_t v[4] = {};
+    for (int i = 0; i < 16; ++i)
+        if (at + i < k) {
+            const uint32_t b = (uint32_t)(uint8_t)row[at + i] << (8 * (i & 3));
+            if (i < 4) v[0] |= b;
+            else if (i < 8) v[1] |= b;
+            else if (i < 12) v[2] |= b;
+            else v[3] |= b;
+        }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-template <typename X, int MT, bool ROWS_OUT>
-__global__ void __launch_bounds__(TK_THREADS) k_token(const TokenParams p)
+template <typename X, int MT>
+__global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
 {
-    constexpr int U = 8;
     extern __shared__ __align__(16) uint8_t smem[];
     const int kpad = (p.k + 15) / 16 * 16, S = 1 << p.log_s;
     int8_t *xq = reinterpret_cast<int8_t *>(smem);                         // [MT][kpad]
     float *xs = reinterpret_cast<float *>(smem + MT * kpad);               // [MT]
     int32_t *red = reinterpret_cast<int32_t *>(xs + MT);                   // [per_cta][S][MT]
     uint32_t *tops = reinterpret_cast<uint32_t *>(red + (p.per_cta << p.log_s) * MT);   // [warps]
-    uint32_t *local = tops + TK_WARPS;                                     // [MT] this CTA's maxima
-    uint32_t *mx = local + MT;                                             // [cluster][MT]
-    float *yb = reinterpret_cast<float *>(mx + TK_CLUSTER * MT);           // [MT][per_cta]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.x * p.per_cta;
     const int64_t t0 = (int64_t)blockIdx.y * MT;
 
-    // this warp's steps: channels slot, slot + abreast, ... of the CTA, in each the vectors of its part
-    const int abreast = TK_WARPS >> p.log_s, slot = warp >> p.log_s, seg = warp & (S - 1);
+    // this warp's channel group and part of K; steps of 32 vectors
+    const int slot = warp >> p.log_s, seg = warp & (S - 1);
     const int kv = kpad / 16, v0 = (int)((int64_t)kv * seg >> p.log_s), v1 = (int)((int64_t)kv * (seg + 1) >> p.log_s);
-    const int per_channel = (((kv + S - 1) >> p.log_s) + 31) / 32;
-    const int items = p.per_cta / abreast * per_channel;
-    int li = 0, lj = 0;                                                    // next step to load
-    auto load = [&]() {
-        const int c = c0 + slot + li * abreast, v = v0 + lj * 32 + lane;
-        const uint4 r = li * per_channel < items && c < p.n && v < v1
-                            ? weight_vec(p.w + (int64_t)c * p.w_stride, v * 16, p.k) : make_uint4(0, 0, 0, 0);
-        if (++lj == per_channel) { lj = 0; ++li; }
-        return r;
-    };
-    uint4 w[U];
+    const int steps = (v1 - v0 + 31) / 32;
+    auto load = [&](uint4(&w)[TK_CH], int c, int v) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = load();
+        for (int i = 0; i < TK_CH; ++i) {
+            w[i] = make_uint4(0, 0, 0, 0);
+            const int8_t *row = p.w + (int64_t)(c + i) * p.w_stride;
+            if (c + i < p.n && v < v1) {
+                // a vector may reach behind its row's end, into the next row, where the tokens are zero
+                if (v * 16 + 16 <= p.k || c + i + 1 < p.n)
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(w[i].x), "=r"(w[i].y), "=r"(w[i].z), "=r"(w[i].w) : "l"(row + v * 16));
+                else w[i] = last_vec(row, v * 16, p.k);
+            }
+        }
+    };
+    next_may_start();
+    previous_done();
+    int c = c0 + slot * TK_CH;                                             // the group's first channel
+    uint4 wa[TK_CH], wb[TK_CH];
+    load(wa, c, v0 + lane);
+    load(wb, c, v0 + 32 + lane);
+    // scale and bias of this thread's first result
+    const int first = c0 + threadIdx.x % p.per_cta;
+    const float ws0 = first < p.n ? p.ws[first] : 0.0f, bias0 = first < p.n && p.bias ? p.bias[first] : 0.0f;
 
     // the tokens
     if (sizeof(X) == 1) {
         const int8_t *x = reinterpret_cast<const int8_t *>(p.x);
         const bool packed = ((uintptr_t)x & 15) == 0 && (p.x_stride & 15) == 0;
-        for (int i = threadIdx.x; i < MT * kv; i += TK_THREADS) {
-            const int t = i / kv, at = i % kv * 16;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (t0 + t < p.rows) {
-                const int8_t *row = x + (t0 + t) * p.x_stride;
-                if (packed && at + 16 <= p.k) {
-                    v = *reinterpret_cast<const uint4 *>(row + at);
-                } else {
-                    int8_t *e = reinterpret_cast<int8_t *>(&v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (at + j < p.k) e[j] = row[at + j];
-                }
-            }
-            *reinterpret_cast<uint4 *>(xq + t * kpad + at) = v;
+#pragma unroll 1
+        for (int t = 0; t < MT; ++t) {
+            const int8_t *row = x + (t0 + t) * p.x_stride;
+            const bool live = t0 + t < p.rows;
+            for (int v = threadIdx.x; v < kv; v += TK_THREADS)
+                *reinterpret_cast<uint4 *>(xq + t * kpad + v * 16) =
+                    !live ? make_uint4(0, 0, 0, 0)
+                          : packed && v * 16 + 16 <= p.k ? *reinterpret_cast<const uint4 *>(row + v * 16)
+                                                         : last_vec(row, v * 16, p.k);
         }
         if (threadIdx.x < MT) xs[threadIdx.x] = t0 + threadIdx.x < p.rows ? p.xs[t0 + threadIdx.x] : 0.0f;
     } else {
@@ -136,39 +135,45 @@ __global__ void __launch_bounds__(TK_THREADS) k_token(const TokenParams p)
             for (int i = 0; i < V::N / 4; ++i) *reinterpret_cast<uint32_t *>(xq + t * kpad + c + 4 * i) = o[i];
         }
     }
-    if (ROWS_OUT && threadIdx.x < MT) local[threadIdx.x] = 0;
     __syncthreads();
-    if (ROWS_OUT) cluster_arrive();                                        // this CTA runs: its memory may be written
 
     // the sums
-    int32_t acc[MT] = {};
-    int ci = 0, cj = 0;
-    for (int it = 0; it < items; it += U) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (it + u >= items) break;
-            const int v = v0 + cj * 32 + lane;
-            const int at = v < v1 ? v * 16 : 0;
+    for (int g = slot; g * TK_CH < p.per_cta; g += TK_WARPS >> p.log_s) {
+        int32_t acc[TK_CH][MT] = {};
+        auto multiply = [&](const uint4(&w)[TK_CH], int v) {
+            const int at = v < v1 ? v * 16 : 0;                            // behind the part's end w is zero
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const uint4 a = *reinterpret_cast<const uint4 *>(xq + t * kpad + at);
-                acc[t] = __dp4a((int)a.x, (int)w[u].x, acc[t]);
-                acc[t] = __dp4a((int)a.y, (int)w[u].y, acc[t]);
-                acc[t] = __dp4a((int)a.z, (int)w[u].z, acc[t]);
-                acc[t] = __dp4a((int)a.w, (int)w[u].w, acc[t]);
-            }
-            w[u] = load();
-            if (++cj == per_channel) {
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int32_t sum = __reduce_add_sync(0xffffffffu, acc[t]);
-                    if (lane == 0) red[(((slot + ci * abreast) << p.log_s) + seg) * MT + t] = sum;
-                    acc[t] = 0;
+                for (int i = 0; i < TK_CH; ++i) {
+                    acc[i][t] = __dp4a((int)a.x, (int)w[i].x, acc[i][t]);
+                    acc[i][t] = __dp4a((int)a.y, (int)w[i].y, acc[i][t]);
+                    acc[i][t] = __dp4a((int)a.z, (int)w[i].z, acc[i][t]);
+                    acc[i][t] = __dp4a((int)a.w, (int)w[i].w, acc[i][t]);
                 }
-                cj = 0;
-                ++ci;
             }
+        };
+        const int next = c + TK_CH * (TK_WARPS >> p.log_s);                // first channel of the next group
+        const bool more = (g + (TK_WARPS >> p.log_s)) * TK_CH < p.per_cta;
+#pragma unroll 1
+        for (int j = 0; j < steps; j += 2) {
+            const int v = v0 + j * 32 + lane;
+            multiply(wa, v);
+            if (j + 2 < steps) load(wa, c, v + 64);
+            else if (more) load(wa, next, v0 + lane);
+            multiply(wb, v + 32);
+            if (j + 2 < steps) load(wb, c, v + 96);
+            else if (more) load(wb, next, v0 + 32 + lane);
         }
+#pragma unroll
+        for (int i = 0; i < TK_CH; ++i)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int32_t sum = __reduce_add_sync(0xffffffffu, acc[i][t]);
+                if (lane == 0) red[(((g * TK_CH + i) << p.log_s) + seg) * MT + t] = sum;
+            }
+        c = next;
     }
     __syncthreads();
 
@@ -178,32 +183,9 @@ __global__ void __launch_bounds__(TK_THREADS) k_token(const TokenParams p)
         if (c >= p.n || t0 + t >= p.rows) continue;
         int32_t sum = 0;
         for (int g = 0; g < S; ++g) sum += red[((ch << p.log_s) + g) * MT + t];
-        const float y = affine(sum, xs[t], p.ws[c], p.bias ? p.bias[c] : 0.0f, p.relu);
-        if constexpr (ROWS_OUT) {
-            yb[i] = y;
-            atomicMax(&local[t], magnitude(y));
-        } else {
-            store_one(p.y, p.y_type, (t0 + t) * p.y_stride + c, y, p.output_scale);
-        }
-    }
-    if constexpr (ROWS_OUT) {
-        __syncthreads();
-        cluster_wait();
-        const uint32_t rank = cluster_ctarank();
-        for (int i = threadIdx.x; i < (int)gridDim.x * MT; i += TK_THREADS) {
-            const uint32_t at = map_to_rank(&mx[rank * MT + i % MT], i / MT);
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(local[i % MT]) : "memory");
-        }
-        cluster_sync();
-        for (int i = threadIdx.x; i < MT * p.per_cta; i += TK_THREADS) {
-            const int t = i / p.per_cta, c = c0 + i % p.per_cta;
-            if (c >= p.n || t0 + t >= p.rows) continue;
-            uint32_t top = 0;
-            for (int r = 0; r < (int)gridDim.x; ++r) top = max(top, mx[r * MT + t]);
-            const RowScale rs = row_scale(top);
-            reinterpret_cast<int8_t *>(p.y)[(t0 + t) * p.y_stride + c] = rs.finite ? (int8_t)quantise_bits(yb[i], rs.r) : 0;
-            if (c == 0) p.y_scales[t0 + t] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
-        }
+        const bool is_first = i == (int)threadIdx.x;
+        const float y = affine(sum, xs[t], is_first ? ws0 : p.ws[c], is_first ? bias0 : p.bias ? p.bias[c] : 0.0f, p.relu);
+        store_one(p.y, p.y_type, (t0 + t) * p.y_stride + c, y, p.output_scale);
     }
 }
 
