@@ -118,9 +118,13 @@ def kernel_launches():
 
 def check(rc, what="sigcomp_b200"):
     """Map a status code to the exception the reference codec raises."""
-    if rc == SC_OK:
-        return
-    msg = last_error() or what
+    if rc != SC_OK:
+        raise_status(rc, last_error(), what)
+
+
+def raise_status(rc, msg, what="sigcomp_b200"):
+    """The exception of a status code other than SC_OK and its message."""
+    msg = msg or what
     if rc == SC_ERR_INVALID_ARGUMENT or rc == SC_ERR_CORRUPT_STREAM:
         raise ValueError(msg)
     if rc == SC_ERR_CAPACITY:

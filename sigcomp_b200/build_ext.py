@@ -1,13 +1,16 @@
-"""Build libsigcomp_b200.so in-tree with nvcc for sm_100a."""
+"""Build libsigcomp_b200.so (nvcc, sm_100a) and its torch binding _int8.so (g++) in-tree."""
 
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libsigcomp_b200.so"
+BINDING = PKG / "_int8.so"
+BINDING_SOURCE = CSRC / "sc_torch.cpp"
 SOURCES = ["sc_capi.cu", "sc_codec.cu", "sc_frames.cu", "sc_int8.cu", "sc_mlp_simple.cu", "sc_mlp_tc.cu", "sc_signal.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
@@ -50,8 +53,31 @@ def _stale():
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 
 
+def build_binding(force=False, verbose=False):
+    """The torch binding of the int8 operators, linked against libsigcomp_b200.so beside it."""
+    header = PKG.parent / "include" / "sigcomp_b200.h"
+    if not force and BINDING.exists() and BINDING.stat().st_mtime > max(
+            f.stat().st_mtime for f in (BINDING_SOURCE, header, Path(__file__))):
+        return BINDING
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    libs = Path(torch.__file__).resolve().parent / "lib"
+    tmp = BINDING.with_suffix(".so.tmp")
+    includes = [sysconfig.get_paths()["include"], *include_paths(), "/usr/local/cuda/include"]
+    cmd = ["/usr/bin/g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           *(a for d in includes for a in ("-isystem", str(d))), str(BINDING_SOURCE), "-o", str(tmp), f"-L{PKG}",
+           f"-l:{LIB.name}", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force=False, verbose=False, jobs=4):
     if not force and not _stale():
+        build_binding(force, verbose)
         return LIB
     objs = []
     build_dir = PKG / "_build"
@@ -87,6 +113,7 @@ def build(force=False, verbose=False, jobs=4):
     subprocess.run([NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-ccbin", "/usr/bin/g++",
                     *objs, "-o", str(tmp), "-lcudart"], check=True)
     os.replace(tmp, LIB)
+    build_binding(force, verbose)
     return LIB
 
 

@@ -395,6 +395,9 @@ void launch(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cuda
     count_launch();
 }
 
+// SMs that plans count on (a B200's), so that a plan and its workspace do not depend on the current device.
+constexpr int kSms = 148;
+
 int sm_count()
 {
     static int counts[64];
@@ -423,7 +426,7 @@ void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t
 {
     const int vecs = (cols + Vec<T>::N - 1) / Vec<T>::N;
     // few rows: one vector a thread, so that a row's latency is one load's
-    const bool few = rows <= 2 * sm_count();
+    const bool few = rows <= 2 * kSms;
     if (vecs <= 32) launch_quantize<T, 32, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 64 && !few) launch_quantize<T, 32, 2, 2>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128 && !few) launch_quantize<T, 32, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
@@ -546,7 +549,7 @@ TokenPlan token_plan(int64_t rows, int64_t n, int64_t k)
 {
     TokenPlan t{0, 0, 0};
     if (rows > 2) return t;
-    const int target = 2 * sm_count();
+    const int target = 2 * kSms;
     // a warp for four channels, or several, down to one 512-byte step of K each, while warps are few
     while (t.log_s < 3 && (n << t.log_s) < (int64_t)target * TK_WARPS * TK_CH && (512 << t.log_s) < k) ++t.log_s;
     const int abreast = (TK_WARPS >> t.log_s) * TK_CH;
@@ -585,7 +588,7 @@ struct MatrixPlan {
 
 MatrixPlan matrix_plan(int64_t rows, int64_t n, int64_t k)
 {
-    const int64_t nkb = (k + PK - 1) / PK, sms = sm_count();
+    const int64_t nkb = (k + PK - 1) / PK, sms = kSms;
     const int64_t units = (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN);
     MatrixPlan best{0, 1};
     double least = 5.0 + (double)((units + sms / 2 - 1) / (sms / 2)) * (0.3 * (double)nkb + 0.9);
