@@ -69,7 +69,8 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top)
 // rint(v r) in the low byte.  The sum with 1.5 * 2^23 has a unit in the last place of one, so the
 // fused multiply-add rounds the exact product to a whole number, ties to even, in one rounding.
 // |v r| <= 127 (1 + 2^-24), so nothing saturates.
-__device__ __forceinline__ uint32_t quantise_bits(float v, float r) { return __float_as_uint(__fmaf_rn(v, r, 12582912.0f)); }
+constexpr float kMagic = 12582912.0f;
+__device__ __forceinline__ uint32_t quantise_bits(float v, float r) { return __float_as_uint(__fmaf_rn(v, r, kMagic)); }
 
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {

@@ -103,19 +103,29 @@ __device__ __forceinline__ void bulk_copy_to(uint32_t dst, const void *src, uint
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// 32 sums of this thread's row -> results; tb: {scale, bias} of the columns
-__device__ __forceinline__ void affine32(const uint32_t (&v)[32], const float4 *tb, float s, int relu, float (&y)[32])
+// 32 sums of this thread's row -> results before ReLU; tb: {scale, bias} of the columns
+__device__ __forceinline__ void affine32(const uint32_t (&v)[32], const float4 *tb, float s, float (&y)[32])
 {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const float4 c = tb[i];
-        y[2 * i] = __fmaf_rn(__fmul_rn(__int2float_rn((int32_t)v[2 * i]), s), c.x, c.y);
-        y[2 * i + 1] = __fmaf_rn(__fmul_rn(__int2float_rn((int32_t)v[2 * i + 1]), s), c.z, c.w);
+        y[2 * i] = affine((int32_t)v[2 * i], s, c.x, c.y, 0);
+        y[2 * i + 1] = affine((int32_t)v[2 * i + 1], s, c.z, c.w, 0);
     }
-    if (relu) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = max_nan(y[i], 0.0f);
-    }
+}
+
+// largest of three, and of three magnitudes; a NaN stays
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_abs_nan(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half)
@@ -165,6 +175,20 @@ __device__ __forceinline__ void staging_free(const PairParams &p, int lane)
     __syncwarp();
 }
 
+// The (row tile, channel block) pairs of one SM pair, `tile_step` tiles and `block_step` blocks further each time.
+struct PairWalk {
+    int tile, block, tile_step, block_step, blocks;
+    __device__ __forceinline__ void next()
+    {
+        tile += tile_step;
+        block += block_step;
+        if (block >= blocks) {
+            block -= blocks;
+            ++tile;
+        }
+    }
+};
+
 template <typename T, int MODE>
 __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ PairParams p)
 {
@@ -178,10 +202,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int nu = (p.n + PN - 1) / PN;                        // units per row tile
-    const int64_t units = (p.rows + 2 * PM - 1) / (2 * PM) * nu;
+    const int tiles = (int)((p.rows + 2 * PM - 1) / (2 * PM));
     // this pair's units: every pairs-th, or, requantising, those of every pairs-th row tile
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-    const int64_t group = REQUANT ? nu : 1;
+    const PairWalk first = REQUANT ? PairWalk{pair, 0, pairs, 0, nu} : PairWalk{pair / nu, pair % nu, pairs / nu, pairs % nu, nu};
+    const int per_step = REQUANT ? nu : 1;                     // units of a step of the walk
     const int nkb = (p.k + PK - 1) / PK;
     const int last_k32 = (p.k - (nkb - 1) * PK + 31) / 32;     // 32-byte steps of the last K block
 
@@ -215,10 +240,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
     if (warp == 0) {
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t g = pair * group; g < units && ok; g += pairs * group)
-            for (int64_t u = g; u < g + group && ok; ++u) {
-                const int row0 = (int)(u / nu) * 2 * PM + (int)rank * PM;
-                const int col0 = (int)(u % nu) * PN + (int)rank * (PN / 2);
+        for (PairWalk g = first; g.tile < tiles && ok; g.next())
+            for (int h = 0; h < per_step && ok; ++h) {
+                const int row0 = g.tile * 2 * PM + (int)rank * PM;
+                const int col0 = (g.block + h) * PN + (int)rank * (PN / 2);
                 for (int kb = 0; kb < nkb; ++kb, ++it) {
                     const int s = it % P_STAGES;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&empty[s], ((it / P_STAGES) & 1) ^ 1)))) break;
@@ -244,8 +269,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
             constexpr uint32_t idesc = idesc_i8(2 * PM, PN);
             uint32_t it = 0, uu = 0;
             bool ok = true;
-            for (int64_t g = pair * group; g < units && ok; g += pairs * group)
-                for (int64_t u = g; u < g + group && ok; ++u, ++uu) {
+            for (PairWalk g = first; g.tile < tiles && ok; g.next())
+                for (int h = 0; h < per_step && ok; ++h, ++uu) {
                     const int ab = uu & 1;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[ab], ((uu >> 1) & 1) ^ 1)))) break;
                     tc_fence_after();
@@ -274,17 +299,26 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
         const int q = warp & 3, grp = (warp - 2) >> 2;
         uint8_t *tile = smem + P_OFF_OUT + (warp - 2) * 4096;
         float2 *tb = (float2 *)(smem + P_OFF_TB + (warp - 2) * P_TB);
-        uint32_t *row_max = (uint32_t *)(smem + P_OFF_MAX);
+        float *row_max = (float *)(smem + P_OFF_MAX);
         const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16) + grp * (PN / 2);
-        uint32_t uu = 0, tiles = 0;
+        uint32_t uu = 0, step = 0;
         bool ok = true;
-        for (int64_t g = pair * group; g < units && ok; g += pairs * group, ++tiles) {
-            const int64_t row0 = g / nu * 2 * PM + rank * PM + q * 32;
-            const float s = row0 + lane < p.rows ? p.xs[row0 + lane] : 0.0f;
-            if (!REQUANT || tiles == 0) {
+        // the row's scale, read a step ahead
+        auto scale_of = [&](const PairWalk &w) {
+            const int64_t r = (int64_t)w.tile * 2 * PM + rank * PM + q * 32 + lane;
+            return r < p.rows ? p.xs[r] : 0.0f;
+        };
+        float s_next = scale_of(first);
+        for (PairWalk g = first; g.tile < tiles && ok; ++step) {
+            const int64_t row0 = (int64_t)g.tile * 2 * PM + rank * PM + q * 32;
+            const int block = g.block;
+            const float s = s_next;
+            g.next();
+            if (g.tile < tiles) s_next = scale_of(g);
+            if (!REQUANT || step == 0) {
                 __syncwarp();
                 for (int h = 0; h < (REQUANT ? nu : 1); ++h) {
-                    const int c0 = (REQUANT ? h : (int)(g % nu)) * PN + grp * (PN / 2);
+                    const int c0 = (block + h) * PN + grp * (PN / 2);
 #pragma unroll
                     for (int i = 0; i < PN / 2; i += 32) {
                         const int c = c0 + i + lane;
@@ -296,7 +330,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
             }
             if constexpr (!REQUANT) {
                 const int ab = uu & 1;
-                const int col0 = (int)(g % nu) * PN + grp * (PN / 2);
+                const int col0 = block * PN + grp * (PN / 2);
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], (uu >> 1) & 1)))) break;
                 ++uu;
                 tc_fence_after();
@@ -310,7 +344,11 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         float y[32];
                         tmem_ld32(lane_base + ab * PN + c + h, v);
                         tmem_ld_wait();
-                        affine32(v, reinterpret_cast<const float4 *>(tb + c + h), s, p.relu, y);
+                        affine32(v, reinterpret_cast<const float4 *>(tb + c + h), s, y);
+                        if (p.relu) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) y[i] = max_nan(y[i], 0.0f);
+                        }
                         if constexpr (MODE == STATIC) {
                             uint32_t o[8];
 #pragma unroll
@@ -339,12 +377,14 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                     if (c + COLS == PN / 2) {                  // the accumulator's last columns are read
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
+                        if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
                     }
                     store_tile<T>(p, tile, row0, col0 + c, lane);
                 }
             } else {
-                uint32_t top = 0;
+                // with ReLU the row's largest result, or 0, is its largest magnitude; the results themselves
+                // stay as they are until they are scaled
+                float top = 0.0f;
                 for (int h = 0; h < nu && ok; ++h) {
                     const int ab = (uu + h) & 1;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], ((uu + h) >> 1) & 1)))) break;
@@ -355,28 +395,33 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         float y[32];
                         tmem_ld32(lane_base + ab * PN + c, v);
                         tmem_ld_wait();
-                        affine32(v, reinterpret_cast<const float4 *>(tb + h * (PN / 2) + c), s, p.relu, y);
+                        affine32(v, reinterpret_cast<const float4 *>(tb + h * (PN / 2) + c), s, y);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            v[i] = __float_as_uint(y[i]);
-                            top = max(top, magnitude(y[i]));
-                        }
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(y[i]);
                         tmem_st32(lane_base + ab * PN + c, v);
+                        if (p.relu) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) top = max3_nan(top, y[i], y[i + 1]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) top = max3_abs_nan(top, y[i], y[i + 1]);
+                        }
                     }
                     tmem_st_wait();
                 }
                 if (!ok) break;
                 // the row's other half of the columns is with the other warp of this quarter, which
                 // cannot be more than one tile ahead: two parities of the buffer are enough
-                uint32_t *mx = row_max + (tiles & 1) * 2 * PM;
+                float *mx = row_max + (step & 1) * 2 * PM;
                 mx[grp * PM + q * 32 + lane] = top;
                 __syncwarp();
-                if (lane == 0) counter_add_release(&max_cnt[grp * 4 + q], 1);
-                if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], tiles + 1)))) break;
-                top = max(top, mx[(grp ^ 1) * PM + q * 32 + lane]);
-                const RowScale rs = row_scale(top);
+                if (elect_one()) counter_add_release(&max_cnt[grp * 4 + q], 1);
+                if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], step + 1)))) break;
+                top = max_nan(top, mx[(grp ^ 1) * PM + q * 32 + lane]);
+                const RowScale rs = row_scale(magnitude(top));
                 if (grp == 0 && row0 + lane < p.rows)
                     p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                const bool all_finite = __all_sync(0xffffffffu, rs.finite);
                 for (int h = 0; h < nu; ++h) {
                     const int ab = (uu + h) & 1;
                     staging_free(p, lane);
@@ -385,20 +430,27 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         uint32_t v[32], o[8];
                         tmem_ld32(lane_base + ab * PN + c, v);
                         tmem_ld_wait();
+                        // ReLU after the multiply-add: results below zero, however far, become 0
+                        const float least = p.relu ? kMagic : -INFINITY;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            o[i] = rs.finite ? pack4(quantise_bits(__uint_as_float(v[4 * i]), rs.r),
-                                                     quantise_bits(__uint_as_float(v[4 * i + 1]), rs.r),
-                                                     quantise_bits(__uint_as_float(v[4 * i + 2]), rs.r),
-                                                     quantise_bits(__uint_as_float(v[4 * i + 3]), rs.r))
-                                             : 0u;
+                        for (int i = 0; i < 8; ++i) {
+                            uint32_t e[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                e[j] = __float_as_uint(fmaxf(__uint_as_float(quantise_bits(__uint_as_float(v[4 * i + j]), rs.r)), least));
+                            o[i] = pack4(e[0], e[1], e[2], e[3]);
+                        }
+                        if (!all_finite && !rs.finite) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) o[i] = 0;
+                        }
                         *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16)) = make_uint4(o[0], o[1], o[2], o[3]);
                         *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16 + 1)) =
                             make_uint4(o[4], o[5], o[6], o[7]);
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
+                    if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
                     store_tile<int8_t>(p, tile, row0, h * PN + grp * (PN / 2), lane);
                 }
                 uu += nu;
