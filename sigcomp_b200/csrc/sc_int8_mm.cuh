@@ -80,17 +80,21 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
+// 16 TMEM lanes x 32 columns, four lanes of the warp sharing a row: register 4 j + 2 i + e of lane l is row
+// 8 i + l / 4, column 8 j + 2 (l % 4) + e.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16])
 {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16x32(uint32_t taddr, const uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
 }
 
 // shared memory of this CTA -> shared memory of another one of the cluster, signalled on its barrier
@@ -103,14 +107,44 @@ __device__ __forceinline__ void bulk_copy_to(uint32_t dst, const void *src, uint
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// 32 sums of this thread's row -> results before ReLU; tb: {scale, bias} of the columns
-__device__ __forceinline__ void affine32(const uint32_t (&v)[32], const float4 *tb, float s, float (&y)[32])
+// Two floats at a time: one instruction on Blackwell, each half rounded by itself.
+struct F2 {
+    float x, y;
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b)
+{
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c)
+{
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+// 32 rows x 32 columns of sums (two halves of 16 rows) -> results before ReLU, in place.  tb: {scale, scale, bias,
+// bias} of the columns' pairs; s: the scales of the thread's four rows.  Four rows share what is read of
+// shared memory: with a row to each thread, reading tb alone took as long as the products of K = 512.
+__device__ __forceinline__ void affine_16x32(uint32_t (&v)[2][16], const float4 *tb, const float (&s)[4])
 {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const float4 c = tb[i];
-        y[2 * i] = affine((int32_t)v[2 * i], s, c.x, c.y, 0);
-        y[2 * i + 1] = affine((int32_t)v[2 * i + 1], s, c.z, c.w, 0);
+    for (int j = 0; j < 4; ++j) {
+        const float4 c = tb[4 * j];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t &a = v[h][4 * j + 2 * i], &b = v[h][4 * j + 2 * i + 1];
+                const F2 f = {__int2float_rn((int32_t)a), __int2float_rn((int32_t)b)};
+                const F2 y = fma2(mul2(f, {s[2 * h + i], s[2 * h + i]}), {c.x, c.y}, {c.z, c.w});
+                a = __float_as_uint(y.x);
+                b = __float_as_uint(y.y);
+            }
     }
 }
 
@@ -298,23 +332,26 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
     } else {
         const int q = warp & 3, grp = (warp - 2) >> 2;
         uint8_t *tile = smem + P_OFF_OUT + (warp - 2) * 4096;
-        float2 *tb = (float2 *)(smem + P_OFF_TB + (warp - 2) * P_TB);
+        float *tb = (float *)(smem + P_OFF_TB + (warp - 2) * P_TB);
         float *row_max = (float *)(smem + P_OFF_MAX);
         const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16) + grp * (PN / 2);
         uint32_t uu = 0, step = 0;
         bool ok = true;
-        // the row's scale, read a step ahead
-        auto scale_of = [&](const PairWalk &w) {
-            const int64_t r = (int64_t)w.tile * 2 * PM + rank * PM + q * 32 + lane;
-            return r < p.rows ? p.xs[r] : 0.0f;
+        // this thread's rows of the warp's 32: rl, rl + 8, rl + 16, rl + 24; their scales are read a step ahead
+        const int rl = lane >> 2, cl = lane & 3;
+        float s_next[4];
+        auto read_scales = [&](const PairWalk &w) {
+            const int64_t r = (int64_t)w.tile * 2 * PM + rank * PM + q * 32 + rl;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_next[i] = r + 8 * i < p.rows ? p.xs[r + 8 * i] : 0.0f;
         };
-        float s_next = scale_of(first);
+        read_scales(first);
         for (PairWalk g = first; g.tile < tiles && ok; ++step) {
             const int64_t row0 = (int64_t)g.tile * 2 * PM + rank * PM + q * 32;
             const int block = g.block;
-            const float s = s_next;
+            const float s[4] = {s_next[0], s_next[1], s_next[2], s_next[3]};
             g.next();
-            if (g.tile < tiles) s_next = scale_of(g);
+            if (g.tile < tiles) read_scales(g);
             if (!REQUANT || step == 0) {
                 __syncwarp();
                 for (int h = 0; h < (REQUANT ? nu : 1); ++h) {
@@ -322,8 +359,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 #pragma unroll
                     for (int i = 0; i < PN / 2; i += 32) {
                         const int c = c0 + i + lane;
-                        tb[h * (PN / 2) + i + lane] =
-                            c < p.n ? make_float2(p.ws[c], p.bias ? p.bias[c] : 0.0f) : make_float2(0.0f, 0.0f);
+                        float *to = tb + h * PN + (i + lane) / 2 * 4 + (lane & 1);
+                        to[0] = c < p.n ? p.ws[c] : 0.0f;
+                        to[2] = c < p.n && p.bias ? p.bias[c] : 0.0f;
                     }
                 }
                 __syncwarp();
@@ -338,41 +376,32 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 #pragma unroll 1
                 for (int c = 0; c < PN / 2; c += COLS) {
                     staging_free(p, lane);
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < COLS; h += 32) {
-                        uint32_t v[32];
-                        float y[32];
-                        tmem_ld32(lane_base + ab * PN + c + h, v);
+                        uint32_t v[2][16];
+                        tmem_ld_16x32(lane_base + ab * PN + c + h, v[0]);
+                        tmem_ld_16x32(lane_base + (16u << 16) + ab * PN + c + h, v[1]);
                         tmem_ld_wait();
-                        affine32(v, reinterpret_cast<const float4 *>(tb + c + h), s, y);
+                        affine_16x32(v, reinterpret_cast<const float4 *>(tb) + (c + h) / 2 + cl, s);
                         if (p.relu) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) y[i] = max_nan(y[i], 0.0f);
+                            for (int i = 0; i < 32; ++i)
+                                v[i / 16][i % 16] = __float_as_uint(max_nan(__uint_as_float(v[i / 16][i % 16]), 0.0f));
                         }
-                        if constexpr (MODE == STATIC) {
-                            uint32_t o[8];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                o[j] = pack4(static_bits(y[4 * j], p.output_scale), static_bits(y[4 * j + 1], p.output_scale),
-                                             static_bits(y[4 * j + 2], p.output_scale),
-                                             static_bits(y[4 * j + 3], p.output_scale));
-                            *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 16)) =
-                                make_uint4(o[0], o[1], o[2], o[3]);
-                            *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 16 + 1)) =
-                                make_uint4(o[4], o[5], o[6], o[7]);
-                        } else if constexpr (sizeof(T) == 4) {
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                *reinterpret_cast<float4 *>(tile + sw128_offset(lane, j)) =
-                                    make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, h / 8 + j)) =
-                                    make_uint4(pack2(y[8 * j], y[8 * j + 1], T()), pack2(y[8 * j + 2], y[8 * j + 3], T()),
-                                               pack2(y[8 * j + 4], y[8 * j + 5], T()),
-                                               pack2(y[8 * j + 6], y[8 * j + 7], T()));
-                        }
+                            for (int i = 0; i < 4; ++i) {
+                                const float y0 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2)]);
+                                const float y1 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2) + 1]);
+                                const uint32_t r = rl + 8 * i, at = (h + 8 * j + 2 * cl) * (uint32_t)sizeof(T);
+                                uint8_t *to = tile + sw128_offset(r, at >> 4) + (at & 15);
+                                if constexpr (MODE == STATIC)
+                                    *reinterpret_cast<uint16_t *>(to) =
+                                        (uint16_t)(static_bits(y0, p.output_scale) | static_bits(y1, p.output_scale) << 8);
+                                else if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(to) = make_float2(y0, y1);
+                                else *reinterpret_cast<uint32_t *>(to) = pack2(y0, y1, T());
+                            }
                     }
                     if (c + COLS == PN / 2) {                  // the accumulator's last columns are read
                         tc_fence_before();
@@ -384,28 +413,28 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
             } else {
                 // with ReLU the row's largest result, or 0, is its largest magnitude; the results themselves
                 // stay as they are until they are scaled
-                float top = 0.0f;
+                float top[4] = {};
                 for (int h = 0; h < nu && ok; ++h) {
                     const int ab = (uu + h) & 1;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], ((uu + h) >> 1) & 1)))) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < PN / 2; c += 32) {
-                        uint32_t v[32];
-                        float y[32];
-                        tmem_ld32(lane_base + ab * PN + c, v);
+                        uint32_t v[2][16];
+                        tmem_ld_16x32(lane_base + ab * PN + c, v[0]);
+                        tmem_ld_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
                         tmem_ld_wait();
-                        affine32(v, reinterpret_cast<const float4 *>(tb + h * (PN / 2) + c), s, y);
+                        affine_16x32(v, reinterpret_cast<const float4 *>(tb + h * PN) + c / 2 + cl, s);
+                        tmem_st_16x32(lane_base + ab * PN + c, v[0]);
+                        tmem_st_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(y[i]);
-                        tmem_st32(lane_base + ab * PN + c, v);
-                        if (p.relu) {
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) top = max3_nan(top, y[i], y[i + 1]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) top = max3_abs_nan(top, y[i], y[i + 1]);
-                        }
+                            for (int i = 0; i < 4; ++i) {
+                                const float y0 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2)]);
+                                const float y1 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2) + 1]);
+                                top[i] = p.relu ? max3_nan(top[i], y0, y1) : max3_abs_nan(top[i], y0, y1);
+                            }
                     }
                     tmem_st_wait();
                 }
@@ -413,32 +442,44 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 // the row's other half of the columns is with the other warp of this quarter, which
                 // cannot be more than one tile ahead: two parities of the buffer are enough
                 float *mx = row_max + (step & 1) * 2 * PM;
-                mx[grp * PM + q * 32 + lane] = top;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                    top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                    if (cl == i) mx[grp * PM + q * 32 + rl + 8 * i] = top[i];
+                }
                 __syncwarp();
                 if (elect_one()) counter_add_release(&max_cnt[grp * 4 + q], 1);
                 if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], step + 1)))) break;
-                top = max_nan(top, mx[(grp ^ 1) * PM + q * 32 + lane]);
-                const RowScale rs = row_scale(magnitude(top));
-                if (grp == 0 && row0 + lane < p.rows)
-                    p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                // from here on a thread has a row of its own: its results lie in 16 bytes at a time
+                const int mine = q * 32 + lane;
+                const RowScale rs = row_scale(magnitude(max_nan(mx[mine], mx[PM + mine])));
+                if (grp == 0 && row0 + lane < p.rows) p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
                 const bool all_finite = __all_sync(0xffffffffu, rs.finite);
+                const float least = p.relu ? kMagic : -INFINITY;
                 for (int h = 0; h < nu; ++h) {
                     const int ab = (uu + h) & 1;
+                    uint32_t v[2][32];                         // the next columns are on their way meanwhile
+                    tmem_ld32(lane_base + ab * PN, v[0]);
                     staging_free(p, lane);
-#pragma unroll 1
+#pragma unroll
                     for (int c = 0; c < PN / 2; c += 32) {
-                        uint32_t v[32], o[8];
-                        tmem_ld32(lane_base + ab * PN + c, v);
+                        const uint32_t(&now)[32] = v[c / 32 % 2];
+                        uint32_t o[8];
                         tmem_ld_wait();
-                        // ReLU after the multiply-add: results below zero, however far, become 0
-                        const float least = p.relu ? kMagic : -INFINITY;
+                        if (c + 32 < PN / 2) tmem_ld32(lane_base + ab * PN + c + 32, v[(c / 32 + 1) % 2]);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            uint32_t e[4];
+                            F2 z[2];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                e[j] = __float_as_uint(fmaxf(__uint_as_float(quantise_bits(__uint_as_float(v[4 * i + j]), rs.r)), least));
-                            o[i] = pack4(e[0], e[1], e[2], e[3]);
+                            for (int j = 0; j < 2; ++j) {
+                                const F2 y = {__uint_as_float(now[4 * i + 2 * j]), __uint_as_float(now[4 * i + 2 * j + 1])};
+                                z[j] = fma2(y, {rs.r, rs.r}, {kMagic, kMagic});
+                                // ReLU after the multiply-add: results below zero, however far, become 0
+                                z[j] = {fmaxf(z[j].x, least), fmaxf(z[j].y, least)};
+                            }
+                            o[i] = pack4(__float_as_uint(z[0].x), __float_as_uint(z[0].y), __float_as_uint(z[1].x),
+                                         __float_as_uint(z[1].y));
                         }
                         if (!all_finite && !rs.finite) {
 #pragma unroll
