@@ -506,13 +506,14 @@ void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y,
     launch(k_pair<T, MODE>, 2 * pairs, P_THREADS, P_SMEM, s, 2, a);
 }
 
-// y (float types, or int8 by one scale) of few int8 rows; `bt` tokens per tile, K split over `split` CTAs
-template <int BT, typename T>
+// y of few int8 rows: float types, int8 by one scale, or (ROWS_OUT) int8 with a scale for each row; BT tokens per
+// tile, K split over `split` CTAs
+template <int BT, bool ROWS_OUT, typename T>
 void launch_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, int split, cudaStream_t s)
 {
     using C = FewCfg<BT>;
     static std::atomic<uint64_t> ready{0};
-    allow_smem(k_few<BT, T>, C::SMEM, ready);
+    allow_smem(k_few<BT, T, ROWS_OUT>, C::SMEM, ready, ROWS_OUT);
     FewParams a;
     a.w = tensor_map(w.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.n, w.stride, PK, 128);
     a.x = tensor_map(x.p, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.k, p.rows, x.stride, PK, BT);
@@ -527,18 +528,21 @@ void launch_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, in
     a.y_stride = y_stride;
     a.y_vec = aligned(y, y_stride * (int64_t)sizeof(T), 4 * sizeof(T));
     a.output_scale = p.output_scale;
-    launch(k_few<BT, T>, dim3((unsigned)split, (unsigned)((p.n + 127) / 128), (unsigned)((p.rows + BT - 1) / BT)), F_THREADS,
-           C::SMEM, s, (unsigned)split, a);
+    a.y_scales = p.y_scales;
+    a.split = split;
+    const unsigned tiles = (unsigned)((p.n + 127) / 128), deep = (unsigned)((p.rows + BT - 1) / BT);
+    const unsigned cluster = ROWS_OUT ? tiles * split : split;
+    launch(k_few<BT, T, ROWS_OUT>, dim3(cluster, ROWS_OUT ? 1 : tiles, deep), F_THREADS, C::SMEM, s, cluster, a);
 }
 
 template <int BT>
 void product_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, void *y, int y_type, int64_t y_stride, int split,
                  cudaStream_t s)
 {
-    if (y_type == SC_TYPE_F32) launch_few<BT>(p, x, xs, w, (float *)y, y_stride, split, s);
-    else if (y_type == SC_TYPE_F16) launch_few<BT>(p, x, xs, w, (__half *)y, y_stride, split, s);
-    else if (y_type == SC_TYPE_BF16) launch_few<BT>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, split, s);
-    else launch_few<BT>(p, x, xs, w, (int8_t *)y, y_stride, split, s);
+    if (y_type == SC_TYPE_F32) launch_few<BT, false>(p, x, xs, w, (float *)y, y_stride, split, s);
+    else if (y_type == SC_TYPE_F16) launch_few<BT, false>(p, x, xs, w, (__half *)y, y_stride, split, s);
+    else if (y_type == SC_TYPE_BF16) launch_few<BT, false>(p, x, xs, w, (__nv_bfloat16 *)y, y_stride, split, s);
+    else launch_few<BT, false>(p, x, xs, w, (int8_t *)y, y_stride, split, s);
 }
 
 // How one or two rows run on k_token; per_cta = 0 where they do not.
@@ -585,14 +589,15 @@ void product_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
 //   K = 4,096, N = 4,096: 16 rows 5.9 / 13.8,  400 rows 15.8 / 14.8,  1,000 rows 29.9 / 15.8
 struct MatrixPlan {
     int bt, split;               // k_few's tile and split of K, or bt = 0: k_pair
+    double time;
 };
 
 MatrixPlan matrix_plan(int64_t rows, int64_t n, int64_t k)
 {
     const int64_t nkb = (k + PK - 1) / PK, sms = kSms;
     const int64_t units = (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN);
-    MatrixPlan best{0, 1};
-    double least = 5.0 + (double)((units + sms / 2 - 1) / (sms / 2)) * (0.3 * (double)nkb + 0.9);
+    MatrixPlan best{0, 1, 0};
+    best.time = 5.0 + (double)((units + sms / 2 - 1) / (sms / 2)) * (0.3 * (double)nkb + 0.9);
     const struct { int bt; double fixed, block; } tiles[] = {{16, 2.9, 0.24}, {32, 3.4, 0.25}, {64, 4.3, 0.27}, {128, 6.1, 0.33}};
     for (const auto &t : tiles) {
         const int64_t count = (rows + t.bt - 1) / t.bt * ((n + 127) / 128);
@@ -600,12 +605,23 @@ MatrixPlan matrix_plan(int64_t rows, int64_t n, int64_t k)
         int split = 1;
         while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * count <= sms) split *= 2;
         const double time = (double)((count * split + sms - 1) / sms) * (t.fixed + t.block * (double)((nkb + split - 1) / split));
-        if (time < least) {
-            least = time;
-            best = {t.bt, split};
-        }
+        if (time < best.time) best = {t.bt, split, time};
     }
     return best;
+}
+
+// Requantised rows in one launch of k_few: a cluster of up to sixteen CTAs with all channels of 16 tokens, in one wave.
+// The alternatives are a product in 32 bits and a launch that quantises it, which adds about 2 us, or
+// k_pair.  16 rows, 512 x 512: TODO us against TODO; K = 8,192 stays with the larger split of K.
+MatrixPlan few_rows_plan(int64_t rows, int64_t n, int64_t k)
+{
+    const int64_t nkb = (k + PK - 1) / PK, tiles = (n + 127) / 128, deep = (rows + 15) / 16;
+    MatrixPlan o{0, 1, 1e30};
+    if (tiles > F_MAX_CLUSTER || tiles * deep > kSms) return o;
+    int split = 1;
+    while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * tiles <= F_MAX_CLUSTER && 2 * split * tiles * deep <= kSms)
+        split *= 2;
+    return {16, split, 3.8 + 0.24 * (double)((nkb + split - 1) / split)};
 }
 
 }  // namespace
@@ -632,7 +648,7 @@ static int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 // rows of a float x held in 8 bits, x and w spread where TMA cannot read them, and the product's rows
 // in 32 bits where a launch of their own quantises them.
 struct Plan {
-    bool quantise, spread_x, spread_w, requant;
+    bool quantise, spread_x, spread_w, requant, few_rows;
     TokenPlan t;
     MatrixPlan m;
     int64_t bytes;
@@ -643,12 +659,23 @@ static Plan plan(const Int8Linear &p)
     Plan o{};
     const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
     o.t = token_plan(p.rows, p.n, p.k);
+    if (o.t.per_cta == 0) o.m = matrix_plan(p.rows, p.n, p.k);
+    if (rows_out) {
+        // what the launches without it would take: k_token reads about 6 MB of weights a microsecond
+        const double others = o.t.per_cta > 0 ? 5.0 + (double)p.n * (double)p.k / 6e6
+                              : o.m.bt > 0 || p.n > 2 * PN ? o.m.time + 2.0 : o.m.time;
+        const MatrixPlan f = few_rows_plan(p.rows, p.n, p.k);
+        o.few_rows = f.time < others;
+        if (o.few_rows) {
+            o.m = f;
+            o.t.per_cta = 0;
+        }
+    }
     const bool token = o.t.per_cta > 0;
-    if (!token) o.m = matrix_plan(p.rows, p.n, p.k);
     o.quantise = p.x_type != SC_TYPE_I8 && !token;
     o.spread_x = p.x_type == SC_TYPE_I8 && !token && !p.x_packed;
     o.spread_w = !p.w_packed;
-    o.requant = rows_out && (token || o.m.bt > 0 || p.n > 2 * PN);
+    o.requant = rows_out && !o.few_rows && (token || o.m.bt > 0 || p.n > 2 * PN);
     if (o.quantise) o.bytes += pad(p.rows * 4, 256);
     if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
     if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
@@ -695,7 +722,8 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
         else if (p.x_type == SC_TYPE_F32) product_token<float>(a, o.t, s);
         else if (p.x_type == SC_TYPE_F16) product_token<__half>(a, o.t, s);
         else product_token<__nv_bfloat16>(a, o.t, s);
-    } else if (o.m.bt == 16) product_few<16>(p, x, xs, w, y, y_type, ys, o.m.split, s);
+    } else if (o.few_rows) launch_few<16, true>(p, x, xs, w, (int8_t *)y, ys, o.m.split, s);
+    else if (o.m.bt == 16) product_few<16>(p, x, xs, w, y, y_type, ys, o.m.split, s);
     else if (o.m.bt == 32) product_few<32>(p, x, xs, w, y, y_type, ys, o.m.split, s);
     else if (o.m.bt == 64) product_few<64>(p, x, xs, w, y, y_type, ys, o.m.split, s);
     else if (o.m.bt == 128) product_few<128>(p, x, xs, w, y, y_type, ys, o.m.split, s);

@@ -520,6 +520,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 // once.  No workspace, no counters, one launch.  (Stores to the owner's memory by each thread, and a cluster
 // barrier, took 10,500 clocks for 64 tokens.)
 //
+// Requantised rows (ROWS_OUT): the cluster holds all channels of its tokens, C = n / 128 CTAs with S parts of K
+// each, at most sixteen CTAs; those that own the same tokens exchange their rows' maxima.
+//
 // Warps: 0 TMA producer, 1 MMA issuer, 2-5 epilogue (one for each TMEM lane quarter).
 struct FewParams {
     CUtensorMap w, x;                          // boxes 128 and BT rows x 128 bytes
@@ -529,6 +532,8 @@ struct FewParams {
     void *y;
     int64_t y_stride;
     float output_scale;
+    float *y_scales;
+    int split;                                 // S, a power of two, at most BT / 2
 };
 
 __device__ __forceinline__ void store_one(void *y, int type, int64_t at, float v, float output_scale)
@@ -540,7 +545,8 @@ __device__ __forceinline__ void store_one(void *y, int type, int64_t at, float v
 }
 
 constexpr int F_THREADS = 192;
-constexpr int F_MAX_SPLIT = 8;
+constexpr int F_MAX_SPLIT = 8;                 // CTAs that split a tile's K
+constexpr int F_MAX_CLUSTER = 16;              // CTAs with the same tokens, requantising
 
 template <int BT>
 struct FewCfg {
@@ -550,7 +556,8 @@ struct FewCfg {
     static constexpr int OFF_BAR = OFF_RECV + BT * 128 * 4;
     static constexpr int OFF_TMEM = OFF_BAR + (2 * STAGES + 2) * 8;
     static constexpr int OFF_XS = OFF_TMEM + 16;                       // the tokens' scales
-    static constexpr int SMEM = OFF_XS + BT * 4 + 1024;
+    static constexpr int OFF_MAX = OFF_XS + BT * 4;                    // [C][BT] row maxima
+    static constexpr int SMEM = OFF_MAX + F_MAX_CLUSTER * BT * 4 + 1024;
     static constexpr int TMEM = BT < 32 ? 32 : BT;
     static_assert(SMEM <= 232448 && BT * 128 * 4 <= STAGES * STAGE, "shared memory per CTA");
 };
@@ -562,7 +569,7 @@ __device__ __forceinline__ T result(float y, float output_scale)
     else return from_f32<T>(y);
 }
 
-template <int BT, typename T>
+template <int BT, typename T, bool ROWS_OUT>
 __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ FewParams p)
 {
     using C = FewCfg<BT>;
@@ -574,9 +581,11 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
     int32_t *recv = (int32_t *)(smem + C::OFF_RECV);
     float *xs = (float *)(smem + C::OFF_XS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int S = gridDim.x;                                           // the cluster: x is the split, a power of two
-    const int part = blockIdx.x, own = BT / S;                         // at most BT / 2 parts
-    const int c0 = blockIdx.y * 128;
+    const int S = p.split, own = BT / S;
+    // the cluster is the grid's x: the parts of K, and requantising those of every channel tile
+    const int part = blockIdx.x & (S - 1), tile0 = blockIdx.x - part;
+    const int c0 = (ROWS_OUT ? tile0 / S : blockIdx.y) * 128;
+    const bool alone = gridDim.x == 1;
     const int64_t t0 = (int64_t)blockIdx.z * BT;
     const int nkb_all = (p.k + PK - 1) / PK;
     const int kb0 = (int)((int64_t)nkb_all * part / S), kb1 = (int)((int64_t)nkb_all * (part + 1) / S);
@@ -601,7 +610,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (S > 1) cluster_arrive();                                       // this CTA runs: its memory may be written
+    if (!alone) cluster_arrive();                                      // this CTA runs: its memory may be written
     const uint32_t tmem = *tmem_slot;
     next_may_start();
     previous_done();
@@ -626,7 +635,8 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             spin_ns(100000);
         }
         __syncwarp();
-        if (S > 1) cluster_wait();
+        if (!alone) cluster_wait();
+        if (ROWS_OUT && !alone) cluster_sync();                            // the rows' maxima
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_i8(128, BT);
         uint32_t it = 0;
@@ -647,13 +657,14 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
         }
         if (elect_one()) mma_commit(done);                             // after every MMA above, given up or not
         __syncwarp();
-        if (S > 1) cluster_wait();
+        if (!alone) cluster_wait();
+        if (ROWS_OUT && !alone) cluster_sync();                            // the rows' maxima
     } else {
         // a channel is a lane of TMEM; tokens are the columns
         const int q = warp & 3;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
         for (int i = threadIdx.x - 64; i < BT; i += 128) xs[i] = t0 + i < p.rows ? p.xs[t0 + i] : 0.0f;
-        if (S == 1) {
+        if (!ROWS_OUT && S == 1) {
             const int ch = c0 + q * 32 + lane;
             const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
             asm volatile("bar.sync 1, 128;" ::: "memory");             // the scales are there: warps 2-5, none has left
@@ -702,32 +713,34 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             tc_fence_before();
             fence_proxy_async_smem();
             asm volatile("bar.sync 1, 128;" ::: "memory");             // warps 2-5; none has left
-            cluster_wait();                                            // every CTA of the cluster runs
-            if (warp == 2 && elect_one()) {
-                for (int r = 1; r < S; ++r) {                          // to each owner, a different one first
-                    const int to = (part + r) & (S - 1);
-                    bulk_copy_to(map_to_rank(recv + (part < to ? part : part - 1) * own * 128, (uint32_t)to),
-                                 (int32_t *)smem + to * own * 128, (uint32_t)(own * 128 * 4), map_to_rank(got, (uint32_t)to));
+            if (!alone) cluster_wait();                                // every CTA of the cluster runs
+            if (S > 1) {
+                if (warp == 2 && elect_one()) {
+                    for (int r = 1; r < S; ++r) {                      // to each owner, a different one first
+                        const int to = (part + r) & (S - 1);
+                        bulk_copy_to(map_to_rank(recv + (part < to ? part : part - 1) * own * 128, (uint32_t)(tile0 + to)),
+                                     (int32_t *)smem + to * own * 128, (uint32_t)(own * 128 * 4),
+                                     map_to_rank(got, (uint32_t)(tile0 + to)));
+                    }
                 }
+                __syncwarp();
+                mbar_wait_cluster(got, 0);
+                __syncwarp();
             }
-            __syncwarp();
-            mbar_wait_cluster(got, 0);
-            __syncwarp();
-#pragma unroll 2
-            for (int j = warp - 2; j < own; j += 4) {
-                const int64_t r = t0 + part * own + j;
+            auto results = [&](int j, float(&y)[4]) {
                 int4 sum = *reinterpret_cast<const int4 *>((const int32_t *)smem + (part * own + j) * 128 + 4 * lane);
                 for (int i = 0; i < S - 1; ++i) {
                     const int4 o = *reinterpret_cast<const int4 *>(recv + (i * own + j) * 128 + 4 * lane);
                     sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
                 }
-                if (r >= p.rows) continue;
                 const float s = xs[part * own + j];
+                y[0] = affine(sum.x, s, t[0], b[0], p.relu);
+                y[1] = affine(sum.y, s, t[1], b[1], p.relu);
+                y[2] = affine(sum.z, s, t[2], b[2], p.relu);
+                y[3] = affine(sum.w, s, t[3], b[3], p.relu);
+            };
+            auto store4 = [&](int64_t r, const T(&o)[4]) {
                 T *to = reinterpret_cast<T *>(p.y) + r * p.y_stride + ch;
-                __align__(16) T o[4] = {result<T>(affine(sum.x, s, t[0], b[0], p.relu), p.output_scale),
-                                        result<T>(affine(sum.y, s, t[1], b[1], p.relu), p.output_scale),
-                                        result<T>(affine(sum.z, s, t[2], b[2], p.relu), p.output_scale),
-                                        result<T>(affine(sum.w, s, t[3], b[3], p.relu), p.output_scale)};
                 if (p.y_vec && ch + 4 <= p.n) {
                     if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(o);
                     else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(to) = *reinterpret_cast<const uint2 *>(o);
@@ -737,11 +750,57 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
                     for (int i = 0; i < 4; ++i)
                         if (ch + i < p.n) to[i] = o[i];
                 }
+            };
+            const int64_t first = t0 + part * own;                     // the CTA's first own token
+            if constexpr (!ROWS_OUT) {
+#pragma unroll 2
+                for (int j = warp - 2; j < own; j += 4) {
+                    float y[4];
+                    results(j, y);
+                    if (first + j >= p.rows) continue;
+                    __align__(16) T o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = result<T>(y[i], p.output_scale);
+                    store4(first + j, o);
+                }
+            } else {
+                float y[BT / 4][4];
+                uint32_t *mx = (uint32_t *)(smem + C::OFF_MAX);
+                const int tiles = gridDim.x / S;
+#pragma unroll
+                for (int u = 0; u < BT / 4; ++u) {
+                    const int j = warp - 2 + 4 * u;
+                    if (j >= own) break;
+                    results(j, y[u]);
+                    uint32_t top = 0;                                  // channels behind the last one are 0, or NaN with the row
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top = max(top, magnitude(y[u][i]));
+                    top = __reduce_max_sync(0xffffffffu, top);
+                    if (lane < tiles) {
+                        const uint32_t at = map_to_rank(mx + tile0 / S * BT + j, (uint32_t)(lane * S + part));
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(top) : "memory");
+                    }
+                }
+                if (!alone) cluster_sync();
+                else __syncwarp();
+#pragma unroll
+                for (int u = 0; u < BT / 4; ++u) {
+                    const int j = warp - 2 + 4 * u;
+                    if (j >= own || first + j >= p.rows) break;
+                    uint32_t top = 0;
+                    for (int i = 0; i < tiles; ++i) top = max(top, mx[i * BT + j]);
+                    const RowScale rs = row_scale(top);
+                    __align__(4) T o[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[i] = rs.finite ? (T)quantise_bits(y[u][i], rs.r) : (T)0;
+                    store4(first + j, o);
+                    if (tile0 == 0 && lane == 0) p.y_scales[first + j] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                }
             }
         }
     }
     __syncthreads();
-    if (S > 1) cluster_sync();                                         // what this CTA sent has been received
+    if (!ROWS_OUT && !alone) cluster_sync();                           // what this CTA sent has been received
     if (warp == 1) {
         mbar_wait_cluster_drain(done, 0);
         tc_fence_after();
