@@ -581,47 +581,83 @@ void product_token(const TokenParams &a, const TokenPlan &t, cudaStream_t s)
     else launch_token<X, 2>(a, t, s);
 }
 
-// Which kernel multiplies more than two rows, from the time in microseconds that each is expected to take:
-// so many waves of CTAs, each of them a start and an end plus its K blocks.  Fitted to measurements at 1 to
-// 3,000 rows of seven layers (512 x 512 to 8,192 x 2,048); among them, k_few against k_pair:
-//   K = 512, N = 512:     16 rows 3.4 / 5.9,  1,000 rows 4.5 / 6.5,  3,000 rows 7.9 / 6.6
-//   K = 8,192, N = 512:   16 rows 4.9 / 22,  1,000 rows 11.9 / 23,  3,000 rows 24.1 / 23.4
-//   K = 4,096, N = 4,096: 16 rows 5.9 / 13.8,  400 rows 15.8 / 14.8,  1,000 rows 29.9 / 15.8
-struct MatrixPlan {
-    int bt, split;               // k_few's tile and split of K, or bt = 0: k_pair
+// Clusters of k_few, one CTA to an SM, that fit a B200 at once (cudaOccupancyMaxActiveClusters; a cluster lies
+// within a group of 14 to 20 SMs).
+int cluster_room(int ctas)
+{
+    return ctas == 1 ? 148 : ctas == 2 ? 74 : ctas == 3 ? 45 : ctas == 4 ? 33 : ctas == 5 ? 26 : ctas == 6 ? 22
+           : ctas <= 9 ? 15 : ctas == 10 ? 11 : 7;
+}
+
+// What multiplies a number of rows: the kernel, its tile and split, whether the rows are quantised by a launch of
+// their own, and the time in microseconds that it is expected to take.
+struct Way {
+    enum { TOKEN, FEW, FEW_ROWS, PAIRS, PAIRS_ROWS } kernel;
+    int bt, split;
+    TokenPlan t;
+    bool requant;
     double time;
 };
 
-MatrixPlan matrix_plan(int64_t rows, int64_t n, int64_t k)
+// The way that is expected to take least.  The times are so many waves of CTAs, each of them a start and an end plus
+// its K blocks, and about 2 us for a launch that quantises rows; fitted to measurements at 1 to 20,480 rows of
+// seven layers (512 x 512 to 8,192 x 2,048).  Among them, k_few against k_pair:
+//   K = 512, N = 512:     16 rows 3.4 / 5.9,  1,000 rows 4.5 / 6.5,  3,000 rows 7.9 / 6.2
+//   K = 8,192, N = 512:   16 rows 5.2 / 22,  1,000 rows 12.1 / 23,  3,000 rows 24.1 / 22.8
+//   K = 4,096, N = 4,096: 16 rows 6.0 / 13.8,  400 rows 15.8 / 14.4,  1,000 rows 29.9 / 15.3
+// and, requantised, one launch against two: 16 rows of 512 x 512 3.8 / 5.9, of 8,192 x 512 9.1 / 6.3.
+Way choose(int64_t rows, int64_t n, int64_t k, bool rows_out)
 {
-    const int64_t nkb = (k + PK - 1) / PK, sms = kSms;
-    const int64_t units = (rows + 2 * PM - 1) / (2 * PM) * ((n + PN - 1) / PN);
-    MatrixPlan best{0, 1, 0};
-    best.time = 5.0 + (double)((units + sms / 2 - 1) / (sms / 2)) * (0.3 * (double)nkb + 0.9);
-    const struct { int bt; double fixed, block; } tiles[] = {{16, 2.9, 0.24}, {32, 3.4, 0.25}, {64, 4.3, 0.27}, {128, 6.1, 0.33}};
-    for (const auto &t : tiles) {
-        const int64_t count = (rows + t.bt - 1) / t.bt * ((n + 127) / 128);
-        if (count > 4 * sms || (t.bt > 16 && rows <= t.bt / 2)) continue;
-        int split = 1;
-        while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * count <= sms) split *= 2;
-        const double time = (double)((count * split + sms - 1) / sms) * (t.fixed + t.block * (double)((nkb + split - 1) / split));
-        if (time < best.time) best = {t.bt, split, time};
+    const int64_t nkb = (k + PK - 1) / PK, pairs = kSms / 2;
+    const int64_t tiles = (rows + 2 * PM - 1) / (2 * PM), blocks = (n + PN - 1) / PN, channels = (n + 127) / 128;
+    auto waves = [](int64_t count, int64_t room) { return (double)((count + room - 1) / room); };
+    // a product in 32 bits is written, read and quantised
+    const double extra = rows_out ? 2.0 + (double)rows * (double)n * 9.0 / 5e6 : 0.0;
+    const TokenPlan t = token_plan(rows, n, k);
+    Way best{Way::PAIRS, 0, 1, t, rows_out, 4.2 + waves(tiles * blocks, pairs) * (0.3 * (double)nkb + 0.5) + extra};
+    auto offer = [&](decltype(best.kernel) kernel, int bt, int split, bool requant, double time) {
+        if (time < best.time) best = {kernel, bt, split, t, requant, time};
+    };
+    // k_token reads about 6 MB of weights a microsecond
+    if (t.per_cta > 0) offer(Way::TOKEN, 0, 1, rows_out, 3.0 + (double)n * (double)k / 6e6 + extra);
+    const struct { int bt; double fixed, block; } sizes[] = {{16, 2.9, 0.24}, {32, 3.4, 0.25}, {64, 4.3, 0.27}, {128, 6.1, 0.33}};
+    for (const auto &z : sizes) {
+        const int64_t count = (rows + z.bt - 1) / z.bt * channels;
+        if (count > 4 * kSms || rows <= 2 || (z.bt > 16 && rows <= z.bt / 2)) continue;
+        for (int split = 1; split <= F_MAX_SPLIT && split <= nkb; split *= 2)
+            offer(Way::FEW, z.bt, split, rows_out,
+                  waves(count, cluster_room(split)) * (z.fixed + z.block * (double)((nkb + split - 1) / split)) + extra);
+    }
+    if (rows_out) {
+        const int64_t deep = (rows + 15) / 16;
+        for (int split = 1; split <= F_MAX_SPLIT && split <= nkb && split * channels <= F_MAX_CLUSTER; split *= 2)
+            if (deep <= cluster_room((int)(split * channels)))
+                offer(Way::FEW_ROWS, 16, split, false, 3.2 + 0.24 * (double)((nkb + split - 1) / split));
+        if (blocks <= 2)
+            offer(Way::PAIRS_ROWS, 0, 1, false, 4.2 + waves(tiles, pairs) * ((double)blocks * 0.3 * (double)nkb + 2.9));
     }
     return best;
 }
 
-// Requantised rows in one launch of k_few: a cluster of up to sixteen CTAs with all channels of 16 tokens, in one wave.
-// The alternatives are a product in 32 bits and a launch that quantises it, which adds about 2 us, or
-// k_pair.  16 rows, 512 x 512: TODO us against TODO; K = 8,192 stays with the larger split of K.
-MatrixPlan few_rows_plan(int64_t rows, int64_t n, int64_t k)
+// The rows of a call, cut in two where the pair kernel's last wave would leave most SMs idle for the time that its
+// K takes: 20,480 rows of 8,192 x 512 requantised, 97 us in two waves, TODO us as one wave and 1,536 rows apart.
+struct Ways {
+    int64_t cut;                 // rows of the first way; the others take the second
+    Way way[2];
+};
+
+Ways cut_rows(int64_t rows, int64_t n, int64_t k, bool rows_out)
 {
-    const int64_t nkb = (k + PK - 1) / PK, tiles = (n + 127) / 128, deep = (rows + 15) / 16;
-    MatrixPlan o{0, 1, 1e30};
-    if (tiles > F_MAX_CLUSTER || tiles * deep > kSms) return o;
-    int split = 1;
-    while (split < F_MAX_SPLIT && 2 * split <= nkb && 2 * split * tiles <= F_MAX_CLUSTER && 2 * split * tiles * deep <= kSms)
-        split *= 2;
-    return {16, split, 3.8 + 0.24 * (double)((nkb + split - 1) / split)};
+    Ways o{rows, {choose(rows, n, k, rows_out), {}}};
+    const Way &all = o.way[0];
+    if (all.kernel != Way::PAIRS && all.kernel != Way::PAIRS_ROWS) return o;
+    const int64_t tiles = (rows + 2 * PM - 1) / (2 * PM), blocks = (n + PN - 1) / PN, pairs = kSms / 2;
+    const int64_t per_tile = all.kernel == Way::PAIRS_ROWS ? 1 : blocks;
+    const int64_t full = tiles * per_tile / pairs * pairs / per_tile * 2 * PM;      // rows of the full waves
+    if (full <= 0 || full >= rows) return o;
+    const Way main = choose(full, n, k, rows_out), rest = choose(rows - full, n, k, rows_out);
+    if (main.time + rest.time < all.time) o = {full, {main, rest}};
+    return o;
 }
 
 }  // namespace
@@ -648,42 +684,65 @@ static int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 // rows of a float x held in 8 bits, x and w spread where TMA cannot read them, and the product's rows
 // in 32 bits where a launch of their own quantises them.
 struct Plan {
-    bool quantise, spread_x, spread_w, requant, few_rows;
-    TokenPlan t;
-    MatrixPlan m;
+    Ways ways;
+    bool quantise, spread_x, spread_w;
+    int64_t wide;                // rows of the product in 32 bits
     int64_t bytes;
 };
 
 static Plan plan(const Int8Linear &p)
 {
     Plan o{};
-    const bool rows_out = p.y_type == SC_TYPE_I8 && p.y_scales;
-    o.t = token_plan(p.rows, p.n, p.k);
-    if (o.t.per_cta == 0) o.m = matrix_plan(p.rows, p.n, p.k);
-    if (rows_out) {
-        // what the launches without it would take: k_token reads about 6 MB of weights a microsecond
-        const double others = o.t.per_cta > 0 ? 5.0 + (double)p.n * (double)p.k / 6e6
-                              : o.m.bt > 0 || p.n > 2 * PN ? o.m.time + 2.0 : o.m.time;
-        const MatrixPlan f = few_rows_plan(p.rows, p.n, p.k);
-        o.few_rows = f.time < others;
-        if (o.few_rows) {
-            o.m = f;
-            o.t.per_cta = 0;
-        }
-    }
-    const bool token = o.t.per_cta > 0;
+    o.ways = cut_rows(p.rows, p.n, p.k, p.y_type == SC_TYPE_I8 && p.y_scales);
+    const Way *w = o.ways.way;
+    const bool token = w[0].kernel == Way::TOKEN;
     o.quantise = p.x_type != SC_TYPE_I8 && !token;
     o.spread_x = p.x_type == SC_TYPE_I8 && !token && !p.x_packed;
     o.spread_w = !p.w_packed;
-    o.requant = rows_out && !o.few_rows && (token || o.m.bt > 0 || p.n > 2 * PN);
+    o.wide = w[0].requant ? o.ways.cut : 0;
+    if (o.ways.cut < p.rows && w[1].requant) o.wide = std::max(o.wide, p.rows - o.ways.cut);
     if (o.quantise) o.bytes += pad(p.rows * 4, 256);
     if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
     if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
-    if (o.requant) o.bytes += pad(p.rows * p.n * 4, 256);
+    o.bytes += pad(o.wide * p.n * 4, 256);
     return o;
 }
 
 int64_t int8_linear_workspace(const Int8Linear &p) { return plan(p).bytes; }
+
+// p's rows, x and w being int8 rows that TMA can read (k_token: as they are); `wide` takes a product in 32 bits
+static void multiply(const Int8Linear &p, const Way &way, Rows8 x, const float *xs, Rows8 w, float *wide, cudaStream_t s)
+{
+    void *y = way.requant ? wide : p.y;
+    const int y_type = way.requant ? SC_TYPE_F32 : p.y_type;
+    const int64_t ys = way.requant ? p.n : p.y_stride;
+    switch (way.kernel) {
+    case Way::TOKEN: {
+        const TokenParams a{p.x, p.x_stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k, p.relu,
+                            y_type, y, ys, p.output_scale, way.t.per_cta, way.t.log_s};
+        if (p.x_type == SC_TYPE_I8) product_token<int8_t>(a, way.t, s);
+        else if (p.x_type == SC_TYPE_F32) product_token<float>(a, way.t, s);
+        else if (p.x_type == SC_TYPE_F16) product_token<__half>(a, way.t, s);
+        else product_token<__nv_bfloat16>(a, way.t, s);
+        break;
+    }
+    case Way::FEW:
+        if (way.bt == 16) product_few<16>(p, x, xs, w, y, y_type, ys, way.split, s);
+        else if (way.bt == 32) product_few<32>(p, x, xs, w, y, y_type, ys, way.split, s);
+        else if (way.bt == 64) product_few<64>(p, x, xs, w, y, y_type, ys, way.split, s);
+        else product_few<128>(p, x, xs, w, y, y_type, ys, way.split, s);
+        break;
+    case Way::FEW_ROWS: launch_few<16, true>(p, x, xs, w, (int8_t *)y, ys, way.split, s); break;
+    case Way::PAIRS_ROWS: product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, ys, s); break;
+    case Way::PAIRS:
+        if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, ys, s);
+        else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, ys, s);
+        else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, ys, s);
+        else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, ys, s);
+        break;
+    }
+    if (way.requant) quantize((const float *)y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+}
 
 void int8_linear(const Int8Linear &p, cudaStream_t s)
 {
@@ -711,28 +770,21 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
         x = spread(x.p, p.rows, x.stride);
     }
     if (o.spread_w) w = spread(p.w, p.n, p.w_stride);
-    // the product itself: to y, or in 32 bits to the workspace
-    void *y = o.requant ? take(p.rows * p.n * 4) : p.y;
-    const int y_type = o.requant ? SC_TYPE_F32 : p.y_type;
-    const int64_t ys = o.requant ? p.n : p.y_stride;
-    if (o.t.per_cta > 0) {
-        const TokenParams a{p.x, p.x_stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k, p.relu,
-                            y_type, y, ys, p.output_scale, o.t.per_cta, o.t.log_s};
-        if (p.x_type == SC_TYPE_I8) product_token<int8_t>(a, o.t, s);
-        else if (p.x_type == SC_TYPE_F32) product_token<float>(a, o.t, s);
-        else if (p.x_type == SC_TYPE_F16) product_token<__half>(a, o.t, s);
-        else product_token<__nv_bfloat16>(a, o.t, s);
-    } else if (o.few_rows) launch_few<16, true>(p, x, xs, w, (int8_t *)y, ys, o.m.split, s);
-    else if (o.m.bt == 16) product_few<16>(p, x, xs, w, y, y_type, ys, o.m.split, s);
-    else if (o.m.bt == 32) product_few<32>(p, x, xs, w, y, y_type, ys, o.m.split, s);
-    else if (o.m.bt == 64) product_few<64>(p, x, xs, w, y, y_type, ys, o.m.split, s);
-    else if (o.m.bt == 128) product_few<128>(p, x, xs, w, y, y_type, ys, o.m.split, s);
-    else if (y_type == SC_TYPE_I8 && p.y_scales) product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, ys, s);
-    else if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, ys, s);
-    else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, ys, s);
-    else if (y_type == SC_TYPE_F16) product_pairs<__half, PLAIN>(p, x, xs, w, (__half *)y, ys, s);
-    else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, ys, s);
-    if (o.requant) quantize((const float *)y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+    float *wide = (float *)ws;
+    Int8Linear part = p;
+    part.rows = o.ways.cut;
+    multiply(part, o.ways.way[0], x, xs, w, wide, s);
+    if (o.ways.cut < p.rows) {
+        const int64_t cut = o.ways.cut, e = p.y_type == SC_TYPE_F32 ? 4 : p.y_type == SC_TYPE_I8 ? 1 : 2;
+        part.rows = p.rows - cut;
+        part.y = (uint8_t *)p.y + cut * p.y_stride * e;
+        part.y_scales = p.y_scales ? p.y_scales + cut : nullptr;
+        // never k_token on a float x: the rest has more than two rows, or x is int8 by now
+        part.x = x.p + cut * x.stride;
+        part.x_type = SC_TYPE_I8;
+        part.x_stride = x.stride;
+        multiply(part, o.ways.way[1], {x.p + cut * x.stride, x.stride}, xs + cut, w, wide, s);
+    }
 }
 
 int int8_device_error()
