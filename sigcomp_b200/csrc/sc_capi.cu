@@ -55,12 +55,16 @@ namespace {
 struct DeviceGuard {
     int prev = -1;
     cudaError_t err = cudaSuccess;
+    bool moved = false;
     explicit DeviceGuard(int dev) {
         cudaGetDevice(&prev);
-        if (prev != dev) err = cudaSetDevice(dev);
+        if (prev != dev) {
+            err = cudaSetDevice(dev);
+            moved = true;
+        }
     }
     ~DeviceGuard() {
-        if (prev >= 0) cudaSetDevice(prev);
+        if (moved && prev >= 0) cudaSetDevice(prev);
     }
 };
 
