@@ -532,7 +532,7 @@ void launch_few(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, in
     a.split = split;
     const unsigned tiles = (unsigned)((p.n + 127) / 128), deep = (unsigned)((p.rows + BT - 1) / BT);
     const unsigned cluster = ROWS_OUT ? tiles * split : split;
-    launch(k_few<BT, T, ROWS_OUT>, dim3(cluster, ROWS_OUT ? 1 : tiles, deep), F_THREADS, C::SMEM, s, cluster, a);
+    launch(k_few<BT, T, ROWS_OUT>, dim3(cluster, ROWS_OUT ? 1 : tiles, deep), C::THREADS, C::SMEM, s, cluster, a);
 }
 
 template <int BT>

@@ -523,7 +523,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 // Requantised rows (ROWS_OUT): the cluster holds all channels of its tokens, C = n / 128 CTAs with S parts of K
 // each, at most sixteen CTAs; those that own the same tokens exchange their rows' maxima.
 //
-// Warps: 0 TMA producer, 1 MMA issuer, 2-5 epilogue (one for each TMEM lane quarter).
+// Warps: 0 TMA producer, 1 MMA issuer, then the epilogue: four warps, or from 64 tokens on eight, two for each TMEM lane
+// quarter with half of the tokens each (1,000 rows of 1,024 x 1,024: 6.9 us with four, 6.1 with eight; with 16
+// tokens eight are slower, 3.55 against 3.4).
 struct FewParams {
     CUtensorMap w, x;                          // boxes 128 and BT rows x 128 bytes
     const float *xs, *ws, *bias;
@@ -544,12 +546,14 @@ __device__ __forceinline__ void store_one(void *y, int type, int64_t at, float v
     else reinterpret_cast<int8_t *>(y)[at] = (int8_t)static_bits(v, output_scale);
 }
 
-constexpr int F_THREADS = 192;
 constexpr int F_MAX_SPLIT = 8;                 // CTAs that split a tile's K
 constexpr int F_MAX_CLUSTER = 16;              // CTAs with the same tokens, requantising
 
 template <int BT>
 struct FewCfg {
+    static constexpr int EPI = BT >= 64 ? 8 : 4;                       // epilogue warps
+    static constexpr int GROUPS = EPI / 4, COLS = BT / GROUPS;         // tokens of each group of four
+    static constexpr int THREADS = 32 * (2 + EPI);
     static constexpr int STAGES = BT <= 32 ? 9 : BT == 64 ? 7 : 4;
     static constexpr int STAGE = 128 * PK + BT * PK;
     static constexpr int OFF_RECV = STAGES * STAGE;                    // [S - 1][BT / S][128] sums from the other CTAs
@@ -562,6 +566,10 @@ struct FewCfg {
     static_assert(SMEM <= 232448 && BT * 128 * 4 <= STAGES * STAGE, "shared memory per CTA");
 };
 
+// a barrier of the epilogue's threads, which all reach it
+template <int THREADS>
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
 template <typename T>
 __device__ __forceinline__ T result(float y, float output_scale)
 {
@@ -570,7 +578,7 @@ __device__ __forceinline__ T result(float y, float output_scale)
 }
 
 template <int BT, typename T, bool ROWS_OUT>
-__global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ FewParams p)
+__global__ void __launch_bounds__(FewCfg<BT>::THREADS, 1) k_few(const __grid_constant__ FewParams p)
 {
     using C = FewCfg<BT>;
     extern __shared__ uint8_t smem_raw[];
@@ -661,19 +669,19 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
         if (ROWS_OUT && !alone) cluster_sync();                            // the rows' maxima
     } else {
         // a channel is a lane of TMEM; tokens are the columns
-        const int q = warp & 3;
+        const int q = warp & 3, grp = (warp - 2) >> 2;
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-        for (int i = threadIdx.x - 64; i < BT; i += 128) xs[i] = t0 + i < p.rows ? p.xs[t0 + i] : 0.0f;
+        for (int i = threadIdx.x - 64; i < BT; i += 32 * C::EPI) xs[i] = t0 + i < p.rows ? p.xs[t0 + i] : 0.0f;
         if (!ROWS_OUT && S == 1) {
             const int ch = c0 + q * 32 + lane;
             const float t = ch < p.n ? p.ws[ch] : 0.0f, b = ch < p.n && p.bias ? p.bias[ch] : 0.0f;
-            asm volatile("bar.sync 1, 128;" ::: "memory");             // the scales are there: warps 2-5, none has left
+            epilogue_sync<32 * C::EPI>();                              // the scales are there; no warp has left
             mbar_wait(done, 0);
             __syncwarp();
             tc_fence_after();
-            T *to = reinterpret_cast<T *>(p.y) + t0 * p.y_stride + ch;
+            T *to = reinterpret_cast<T *>(p.y) + (t0 + grp * C::COLS) * p.y_stride + ch;
 #pragma unroll 1
-            for (int j0 = 0; j0 < BT && t0 + j0 < p.rows; j0 += 16) {
+            for (int j0 = grp * C::COLS; j0 < (grp + 1) * C::COLS && t0 + j0 < p.rows; j0 += 16) {
                 uint32_t v[16];
                 tmem_ld16(taddr + j0, v);
                 tmem_ld_wait();
@@ -703,7 +711,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             // the stages are read: their memory takes the sums, token by token
             int32_t *sums = (int32_t *)smem + q * 32 + lane;
 #pragma unroll 1
-            for (int j0 = 0; j0 < BT; j0 += 16) {
+            for (int j0 = grp * C::COLS; j0 < (grp + 1) * C::COLS; j0 += 16) {
                 uint32_t v[16];
                 tmem_ld16(taddr + j0, v);
                 tmem_ld_wait();
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             }
             tc_fence_before();
             fence_proxy_async_smem();
-            asm volatile("bar.sync 1, 128;" ::: "memory");             // warps 2-5; none has left
+            epilogue_sync<32 * C::EPI>();                              // no warp has left
             if (!alone) cluster_wait();                                // every CTA of the cluster runs
             if (S > 1) {
                 if (warp == 2 && elect_one()) {
@@ -754,7 +762,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
             const int64_t first = t0 + part * own;                     // the CTA's first own token
             if constexpr (!ROWS_OUT) {
 #pragma unroll 2
-                for (int j = warp - 2; j < own; j += 4) {
+                for (int j = warp - 2; j < own; j += C::EPI) {
                     float y[4];
                     results(j, y);
                     if (first + j >= p.rows) continue;
@@ -764,12 +772,12 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
                     store4(first + j, o);
                 }
             } else {
-                float y[BT / 4][4];
+                float y[BT / C::EPI][4];
                 uint32_t *mx = (uint32_t *)(smem + C::OFF_MAX);
                 const int tiles = gridDim.x / S;
 #pragma unroll
-                for (int u = 0; u < BT / 4; ++u) {
-                    const int j = warp - 2 + 4 * u;
+                for (int u = 0; u < BT / C::EPI; ++u) {
+                    const int j = warp - 2 + C::EPI * u;
                     if (j >= own) break;
                     results(j, y[u]);
                     uint32_t top = 0;                                  // channels behind the last one are 0, or NaN with the row
@@ -784,8 +792,8 @@ __global__ void __launch_bounds__(F_THREADS, 1) k_few(const __grid_constant__ Fe
                 if (!alone) cluster_sync();
                 else __syncwarp();
 #pragma unroll
-                for (int u = 0; u < BT / 4; ++u) {
-                    const int j = warp - 2 + 4 * u;
+                for (int u = 0; u < BT / C::EPI; ++u) {
+                    const int j = warp - 2 + C::EPI * u;
                     if (j >= own || first + j >= p.rows) break;
                     uint32_t top = 0;
                     for (int i = 0; i < tiles; ++i) top = max(top, mx[i * BT + j]);
