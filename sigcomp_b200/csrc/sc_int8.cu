@@ -117,54 +117,131 @@ template <typename T> struct Vec16 {
 template <> struct Vec<__half> : Vec16<__half> {};
 template <> struct Vec<__nv_bfloat16> : Vec16<__nv_bfloat16> {};
 
-// columns c .. c + N of a row of `cols`, zeros behind its end; ALIGNED: rows start on 16 bytes
-template <typename T, bool ALIGNED>
-__device__ __forceinline__ uint4 load_vec(const T *row, int c, int cols)
+// 16 bytes from byte `at` (0 to 15, a multiple of E) of 32
+template <int E>
+__device__ __forceinline__ uint4 shifted16(const uint4 &a, const uint4 &b, uint32_t at)
 {
-    constexpr int N = Vec<T>::N;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (ALIGNED && c + N <= cols) {
-        raw = *reinterpret_cast<const uint4 *>(row + c);
-    } else {
-        T *e = reinterpret_cast<T *>(&raw);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (c + i < cols) e[i] = row[c + i];
-    }
+    for (int i = 0; i < 6; ++i) w[i] = at & 8 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = at & 4 ? w[i + 1] : w[i];
+    if (E == 4) return make_uint4(w[0], w[1], w[2], w[3]);
+    const uint32_t bits = (at & 3) * 8;
+    return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                      __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// 16 bytes if `in`, else zeros: a predicated load and no branch, so that several are in flight
+__device__ __forceinline__ uint4 load_if(bool in, const void *at)
+{
+    uint4 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+                 "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(at), "r"((int)in) : "memory");
+    return v;
+}
+
+// Element by element what lies within low .. high, zeros in place of the rest
+template <typename T>
+__device__ __forceinline__ uint4 load_elements(const T *at, const T *low, const T *high)
+{
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    T *e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+    for (int i = 0; i < Vec<T>::N; ++i)
+        if (at + i >= low && at + i < high) e[i] = at[i];
     return raw;
 }
 
+// the first `bytes` of 16, zeros behind them
+__device__ __forceinline__ uint4 first_bytes(uint4 v, int bytes)
+{
+    auto keep = [&](uint32_t w, int from) {
+        const int n = bytes - from;
+        return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
+    };
+    return make_uint4(keep(v.x, 0), keep(v.y, 4), keep(v.z, 8), keep(v.w, 12));
+}
+
 // ---- quantise --------------------------------------------------------------------------------
-// A row is read once: T threads hold its 16-byte vectors in registers through the maximum, and a group
-// of threads holds R rows at a time where rows are short, so that enough loads are in flight.  Bound by
-// HBM (e + 1 bytes per element).
+// A row is read once: THREADS threads (a part of a warp, a warp or more) hold its 16-byte vectors in registers through
+// the maximum, R rows at a time where rows are short, so that enough loads are in flight.  Bound by HBM
+// (e + 1 bytes per element).
 template <typename T, int THREADS, int HELD, int R, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ q, int64_t q_stride,
-           float *__restrict__ scales)
+           float *__restrict__ scales, int q_vec)
 {
     constexpr int N = Vec<T>::N;
     constexpr int GROUPS = THREADS < 256 ? 256 / THREADS : 1;      // of THREADS threads, R rows each
     __shared__ uint32_t tops[R][32];
     const int t = threadIdx.x % THREADS, grp = threadIdx.x / THREADS;
     const int64_t row0 = ((int64_t)blockIdx.x * GROUPS + grp) * R;
+    const T *end = x + (rows - 1) * x_stride + cols;
     next_may_start();
     previous_done();
-    uint4 v[R][HELD];
-    uint32_t top[R];
+    // Aligned vectors are requested first, all of them; where rows do not start on 16 bytes (ALIGNED false) a thread has
+    // the one that holds its first column and gets the next from its neighbour, and the last thread of a warp
+    // or part reads that too.  Only addresses within x are read: at its ends element by element.
+    constexpr int LANES = THREADS < 32 ? THREADS : 32;
+    const bool last = (threadIdx.x & (LANES - 1)) == LANES - 1;
+    uint4 v[R][HELD], w[ALIGNED ? 1 : R][ALIGNED ? 1 : HELD];
+    uint32_t top[R], at[R];
+    const T *from[R];
+    int low[R], high[R];                                           // the vectors of a row that lie in x: low to high - 1
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int i = 0; i < R; ++i) {
+        const T *row = x + min(row0 + i, rows - 1) * x_stride;
+        at[i] = ALIGNED ? 0 : (uint32_t)(uintptr_t)row & 15u;
+        from[i] = reinterpret_cast<const T *>(reinterpret_cast<const char *>(row) - at[i]) + t * N;
+        const int live = row0 + i < rows ? cols : -2 * N;          // behind the last row: a row of no columns
+        if (!ALIGNED) {
+            low[i] = from[i] - t * N < x;
+            high[i] = (int)min((int64_t)INT_MAX, (int64_t)(end - (from[i] - t * N)) / N);
+        }
 #pragma unroll
-        for (int h = 0; h < HELD; ++h)
-            v[i][h] = row0 + i < rows ? load_vec<T, ALIGNED>(x + (row0 + i) * x_stride, (h * THREADS + t) * N, cols)
-                                      : make_uint4(0, 0, 0, 0);
+        for (int h = 0; h < HELD; ++h) {
+            const int g = h * THREADS + t, c = g * N;
+            v[i][h] = load_if(ALIGNED ? c + N <= live : g >= low[i] && g < high[i] && c < live + N, from[i] + h * THREADS * N);
+            if (!ALIGNED) w[i][h] = load_if(last && g + 1 < high[i] && c < live, from[i] + (h * THREADS + 1) * N);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int live = row0 + i < rows ? cols : -2 * N;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h) {
+            const int g = h * THREADS + t, c = g * N;
+            const T *p = from[i] + h * THREADS * N;
+            if (ALIGNED) {
+                if (c < live && c + N > live) v[i][h] = load_elements(p, p, p + (live - c));
+            } else {
+                if ((g < low[i] || g >= high[i]) && c < live + N) v[i][h] = load_elements(p, x, end);
+                if (last && g + 1 >= high[i] && c < live) w[i][h] = load_elements(p + N, x, end);
+                const uint4 o = v[i][h];
+                uint4 next = make_uint4(__shfl_down_sync(0xffffffffu, o.x, 1, LANES), __shfl_down_sync(0xffffffffu, o.y, 1, LANES),
+                                        __shfl_down_sync(0xffffffffu, o.z, 1, LANES), __shfl_down_sync(0xffffffffu, o.w, 1, LANES));
+                if (last) next = w[i][h];
+                v[i][h] = shifted16<sizeof(T)>(o, next, at[i]);
+                if (c + N > live) v[i][h] = first_bytes(v[i][h], (live - c) * (int)sizeof(T));
+            }
+        }
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
         uint32_t m = 0;
 #pragma unroll
         for (int h = 0; h < HELD; ++h) m = Vec<T>::top(v[i][h], m);
-        top[i] = __reduce_max_sync(0xffffffffu, Vec<T>::top_bits(m));
-        if (THREADS > 32 && (threadIdx.x & 31) == 0) tops[i][threadIdx.x >> 5] = top[i];
+        m = Vec<T>::top_bits(m);
+        if (THREADS >= 32) {
+            top[i] = __reduce_max_sync(0xffffffffu, m);
+            if (THREADS > 32 && (threadIdx.x & 31) == 0) tops[i][threadIdx.x >> 5] = top[i];
+        } else {
+#pragma unroll
+            for (int d = 1; d < THREADS; d *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+            top[i] = m;
+        }
     }
     if (THREADS > 32) {
         __syncthreads();
@@ -187,9 +264,20 @@ k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, in
             if (!rs.finite)
 #pragma unroll
                 for (int j = 0; j < N / 4; ++j) o[j] = 0;
-            if (ALIGNED && c + N <= cols) {
+            if (q_vec && c + N <= cols) {
                 if constexpr (N == 8) *reinterpret_cast<uint2 *>(qr + c) = make_uint2(o[0], o[1]);
                 else *reinterpret_cast<uint32_t *>(qr + c) = o[0];
+            } else if (q_vec) {                                    // the row's last bytes: four, two and one of them
+                int n = cols - c;
+                if (n >= 4) {
+                    *reinterpret_cast<uint32_t *>(qr + c) = o[0];
+                    o[0] = o[N / 4 - 1];
+                }
+                if (n > 0 && n & 2) {
+                    *reinterpret_cast<uint16_t *>(qr + c + (n & 4)) = (uint16_t)o[0];
+                    o[0] >>= 16;
+                }
+                if (n > 0 && n & 1) qr[c + (n & 6)] = (int8_t)o[0];
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j)
@@ -224,11 +312,13 @@ k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__r
 
 // ---- dequantise ------------------------------------------------------------------------------
 // 16 bytes of results a thread and row, four rows in flight: a block's 256 threads are 2^log_lanes
-// vectors wide.  Bound by HBM (1 + e bytes per element).
+// vectors wide.  Bound by HBM (1 + e bytes per element).  Where y's rows do not start on 16 bytes (ALIGNED false), a
+// row's vectors are those of the addresses, so the first one and the last may be parts, and their bytes
+// of q are read as the three words around them.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256)
 k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__restrict__ scales, float scale, int64_t rows,
-             int cols, T *__restrict__ y, int64_t y_stride, int log_lanes)
+             int cols, T *__restrict__ y, int64_t y_stride, int log_lanes, int q_words)
 {
     constexpr int N = Vec<T>::N, U = 4;
     const int deep = 256 >> log_lanes;                             // rows of one pass
@@ -236,38 +326,64 @@ k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__rest
     const int lane = threadIdx.x & ((1 << log_lanes) - 1);
     next_may_start();
     previous_done();
-    for (int64_t c64 = ((int64_t)blockIdx.y << log_lanes) * N; c64 < cols; c64 += ((int64_t)gridDim.y << log_lanes) * N) {
-        const int c = (int)c64 + lane * N;
-        if (c >= cols) break;
-        if (ALIGNED && c + N <= cols) {
-            uint2 raw[U];
-            float s[U];
+    for (int64_t c64 = ((int64_t)blockIdx.y << log_lanes) * N; c64 < cols + (ALIGNED ? 0 : N - 1);
+         c64 += ((int64_t)gridDim.y << log_lanes) * N) {
+        int c[U];
+        uint32_t raw[U][N / 4];
+        float s[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t r = row0 + u * deep;
-                if (r >= rows) break;
-                const int8_t *at = q + r * q_stride + c;
-                if constexpr (N == 8) raw[u] = *reinterpret_cast<const uint2 *>(at);
-                else raw[u].x = *reinterpret_cast<const uint32_t *>(at);
-                s[u] = scales ? scales[r] : scale;
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row0 + u * deep;
+            c[u] = (int)c64 + lane * N;
+            if (r >= rows) continue;
+            const int8_t *qr = q + r * q_stride;
+            s[u] = scales ? scales[r] : scale;
+            if (ALIGNED) {
+                if (c[u] + N <= cols) {
+                    if constexpr (N == 8) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(qr + c[u]);
+                        raw[u][0] = v.x, raw[u][N / 4 - 1] = v.y;
+                    } else raw[u][0] = *reinterpret_cast<const uint32_t *>(qr + c[u]);
+                }
+            } else {
+                c[u] -= (int)(((uintptr_t)(y + r * y_stride) & 15) / sizeof(T));
+                // the words may reach four bytes behind the vector, which lie in q but at its very end
+                if (q_words && c[u] >= 0 && c[u] + N <= cols && (r + 1 < rows || c[u] + N + 4 <= cols)) {
+                    const uint32_t *at = reinterpret_cast<const uint32_t *>(qr + (c[u] & ~3));
+                    uint32_t w[N / 4 + 1];
+#pragma unroll
+                    for (int i = 0; i <= N / 4; ++i) w[i] = at[i];
+#pragma unroll
+                    for (int i = 0; i < N / 4; ++i) raw[u][i] = __funnelshift_r(w[i], w[i + 1], (c[u] & 3) * 8);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        if (i % 4 == 0) raw[u][i / 4] = 0;
+                        if (c[u] + i >= 0 && c[u] + i < cols) raw[u][i / 4] |= (uint32_t)(uint8_t)qr[c[u] + i] << (8 * (i % 4));
+                    }
+                }
             }
+        }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int64_t r = row0 + u * deep;
-                if (r >= rows) break;
-                const int8_t *e = reinterpret_cast<const int8_t *>(&raw[u]);
-                __align__(16) T out[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i) out[i] = from_f32<T>(__fmul_rn((float)e[i], s[u]));
-                *reinterpret_cast<uint4 *>(y + r * y_stride + c) = *reinterpret_cast<const uint4 *>(out);
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = row0 + u * deep;
+            if (r >= rows) continue;
+            T *yr = y + r * y_stride;
+            if (ALIGNED && c[u] + N > cols) {
+                for (int i = 0; i < N && c[u] + i < cols; ++i)
+                    yr[c[u] + i] = from_f32<T>(__fmul_rn((float)q[r * q_stride + c[u] + i], s[u]));
+                continue;
             }
-        } else {
-            for (int u = 0; u < U; ++u) {
-                const int64_t r = row0 + u * deep;
-                if (r >= rows) break;
-                const float s = scales ? scales[r] : scale;
-                for (int i = 0; i < N && c + i < cols; ++i)
-                    y[r * y_stride + c + i] = from_f32<T>(__fmul_rn((float)q[r * q_stride + c + i], s));
+            __align__(16) T out[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                out[i] = from_f32<T>(__fmul_rn((float)(int8_t)(raw[u][i / 4] >> (8 * (i % 4))), s[u]));
+            if (ALIGNED || (c[u] >= 0 && c[u] + N <= cols)) {
+                *reinterpret_cast<uint4 *>(yr + c[u]) = *reinterpret_cast<const uint4 *>(out);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (c[u] + i >= 0 && c[u] + i < cols) yr[c[u] + i] = out[i];
             }
         }
     }
@@ -416,10 +532,11 @@ void launch_quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, 
 {
     constexpr int PER_BLOCK = (THREADS < 256 ? 256 / THREADS : 1) * R;
     const unsigned g = grid_x((rows + PER_BLOCK - 1) / PER_BLOCK), b = THREADS < 256 ? 256 : THREADS;
-    if (aligned(x, xs * (int64_t)sizeof(T), 16) && aligned(q, qs, Vec<T>::N))
-        launch(k_quantize<T, THREADS, HELD, R, true>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales);
+    const int q_vec = aligned(q, qs, Vec<T>::N);
+    if (aligned(x, xs * (int64_t)sizeof(T), 16))
+        launch(k_quantize<T, THREADS, HELD, R, true>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales, q_vec);
     else
-        launch(k_quantize<T, THREADS, HELD, R, false>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales);
+        launch(k_quantize<T, THREADS, HELD, R, false>, g, b, 0, s, 1, x, rows, cols, xs, q, qs, scales, q_vec);
 }
 
 template <typename T>
@@ -428,13 +545,18 @@ void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t
     const int vecs = (cols + Vec<T>::N - 1) / Vec<T>::N;
     // few rows: one vector a thread, so that a row's latency is one load's
     const bool few = rows <= 2 * kSms;
-    if (vecs <= 32) launch_quantize<T, 32, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    if (vecs <= 1) launch_quantize<T, 1, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 4) launch_quantize<T, 4, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 8) launch_quantize<T, 8, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 16) launch_quantize<T, 16, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 32) launch_quantize<T, 32, 1, 4>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 64 && !few) launch_quantize<T, 32, 2, 2>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128 && !few) launch_quantize<T, 32, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128) launch_quantize<T, 128, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 512 && !few) launch_quantize<T, 128, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024 && few) launch_quantize<T, 1024, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024) launch_quantize<T, 256, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 2048) launch_quantize<T, 512, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 4096) launch_quantize<T, 1024, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else launch(k_quantize_long<T>, grid_x(rows), 1024, 0, s, 1, x, cols, xs, q, qs, scales);
 }
@@ -444,14 +566,16 @@ void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, i
                 cudaStream_t s)
 {
     constexpr int N = Vec<T>::N;
+    const bool al = aligned(q, qs, N) && aligned(y, ys * (int64_t)sizeof(T), 16);
+    const int wide_cols = al ? cols : cols + N - 1;             // a row's vectors may begin before it
     int log_lanes = 0;
-    while (log_lanes < 8 && (N << log_lanes) < cols) ++log_lanes;
+    while (log_lanes < 8 && (N << log_lanes) < wide_cols) ++log_lanes;
     const int64_t deep = (256 >> log_lanes) * 4, wide = (int64_t)N << log_lanes;
-    const dim3 g(grid_x((rows + deep - 1) / deep), (unsigned)std::min<int64_t>((cols + wide - 1) / wide, 65535));
-    if (aligned(q, qs, N) && aligned(y, ys * (int64_t)sizeof(T), 16))
-        launch(k_dequantize<T, true>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes);
+    const dim3 g(grid_x((rows + deep - 1) / deep), (unsigned)std::min<int64_t>((wide_cols + wide - 1) / wide, 65535));
+    if (al) launch(k_dequantize<T, true>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes, 1);
     else
-        launch(k_dequantize<T, false>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes);
+        launch(k_dequantize<T, false>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes,
+               (int)(aligned(q, qs, 4) && qs >= cols));
 }
 
 struct Rows8 {
@@ -704,7 +828,7 @@ static Plan plan(const Int8Linear &p)
     if (o.quantise) o.bytes += pad(p.rows * 4, 256);
     if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
     if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
-    o.bytes += pad(o.wide * p.n * 4, 256);
+    o.bytes += pad(o.wide * pad(p.n, 4) * 4, 256);
     return o;
 }
 
@@ -715,7 +839,7 @@ static void multiply(const Int8Linear &p, const Way &way, Rows8 x, const float *
 {
     void *y = way.requant ? wide : p.y;
     const int y_type = way.requant ? SC_TYPE_F32 : p.y_type;
-    const int64_t ys = way.requant ? p.n : p.y_stride;
+    const int64_t ys = way.requant ? pad(p.n, 4) : p.y_stride;     // rows on 16 bytes, for TMA
     switch (way.kernel) {
     case Way::TOKEN: {
         const TokenParams a{p.x, p.x_stride, xs, w.p, w.stride, p.w_scales, p.bias, p.rows, (int)p.n, (int)p.k, p.relu,
@@ -741,7 +865,7 @@ static void multiply(const Int8Linear &p, const Way &way, Rows8 x, const float *
         else product_pairs<__nv_bfloat16, PLAIN>(p, x, xs, w, (__nv_bfloat16 *)y, ys, s);
         break;
     }
-    if (way.requant) quantize((const float *)y, p.rows, (int)p.n, p.n, (int8_t *)p.y, p.y_stride, p.y_scales, s);
+    if (way.requant) quantize((const float *)y, p.rows, (int)p.n, ys, (int8_t *)p.y, p.y_stride, p.y_scales, s);
 }
 
 void int8_linear(const Int8Linear &p, cudaStream_t s)

@@ -174,11 +174,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16)
 }
 
 // This warp's 32 rows of 128 bytes from its staging tile to y: by TMA, which drops what lies beyond
-// the last row or column, or element by element where y's rows are not 16-byte aligned.
+// the last row or column.  Where y's rows are not 16-byte aligned, eight lanes have a row: they store the 16-byte
+// vectors that its addresses have whole, shifted together from two of the tile's, and then the elements
+// before and after them.
 template <typename T>
 __device__ __forceinline__ void store_tile(const PairParams &p, const uint8_t *tile, int64_t row0, int col0, int lane)
 {
-    constexpr int COLS = 128 / sizeof(T);
     if (p.y_tma) {
         fence_proxy_async_smem();
         __syncwarp();
@@ -187,17 +188,24 @@ __device__ __forceinline__ void store_tile(const PairParams &p, const uint8_t *t
             bulk_commit();
         }
     } else {
+        constexpr int E = 16 / sizeof(T);
         __syncwarp();
-        const int nr = (int)min((int64_t)32, p.rows - row0);
-#pragma unroll 4
-        for (int r = 0; r < nr; ++r)
-#pragma unroll
-            for (int c = lane; c < COLS; c += 32) {
-                const uint32_t off = c * (uint32_t)sizeof(T);
-                if (col0 + c < p.n)
-                    reinterpret_cast<T *>(p.yp)[(row0 + r) * p.y_stride + col0 + c] =
-                        *reinterpret_cast<const T *>(tile + sw128_offset(r, off >> 4) + (off & 15));
+        const int live = (int)min((int64_t)32, p.rows - row0), wide = min(8 * E, p.n - col0);
+        for (int r = lane >> 3; r < live; r += 4) {
+            T *yr = reinterpret_cast<T *>(p.yp) + (row0 + r) * p.y_stride + col0;
+            const int head = (int)((16 - ((uintptr_t)yr & 15)) & 15) / (int)sizeof(T);     // elements before the first vector
+            const int whole = head < wide ? (wide - head) / E : 0;                         // vectors
+            const int j = lane & 7;
+            if (j < whole) {
+                const uint4 a = *reinterpret_cast<const uint4 *>(tile + sw128_offset(r, j));
+                const uint4 b = *reinterpret_cast<const uint4 *>(tile + sw128_offset(r, j < 7 ? j + 1 : 7));
+                *reinterpret_cast<uint4 *>(yr + head + j * E) = shifted16<sizeof(T)>(a, b, head * (uint32_t)sizeof(T));
             }
+            for (int e = j; e < wide - whole * E; e += 8) {
+                const uint32_t c = e < head ? e : e + whole * E, off = c * (uint32_t)sizeof(T);
+                yr[c] = *reinterpret_cast<const T *>(tile + sw128_offset(r, off >> 4) + (off & 15));
+            }
+        }
         __syncwarp();
     }
 }
@@ -336,6 +344,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
         float *row_max = (float *)(smem + P_OFF_MAX);
         const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16) + grp * (PN / 2);
         uint32_t uu = 0, step = 0;
+        int have = -1;                                         // the channel block whose scales and bias are in tb
         bool ok = true;
         // this thread's rows of the warp's 32: rl, rl + 8, rl + 16, rl + 24; their scales are read a step ahead
         const int rl = lane >> 2, cl = lane & 3;
@@ -352,7 +361,8 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
             const float s[4] = {s_next[0], s_next[1], s_next[2], s_next[3]};
             g.next();
             if (g.tile < tiles) read_scales(g);
-            if (!REQUANT || step == 0) {
+            if (block != have) {                               // (requantising, once)
+                have = block;
                 __syncwarp();
                 for (int h = 0; h < (REQUANT ? nu : 1); ++h) {
                     const int c0 = (block + h) * PN + grp * (PN / 2);
@@ -373,8 +383,14 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 ++uu;
                 tc_fence_after();
                 constexpr int COLS = 128 / sizeof(T);          // columns of a staging tile
+                auto release = [&]() {                         // the accumulator's last columns are read
+                    tc_fence_before();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
+                };
+                if (col0 >= p.n) release();
 #pragma unroll 1
-                for (int c = 0; c < PN / 2; c += COLS) {
+                for (int c = 0; c < PN / 2 && col0 + c < p.n; c += COLS) {
                     staging_free(p, lane);
 #pragma unroll 1
                     for (int h = 0; h < COLS; h += 32) {
@@ -403,11 +419,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                                 else *reinterpret_cast<uint32_t *>(to) = pack2(y0, y1, T());
                             }
                     }
-                    if (c + COLS == PN / 2) {                  // the accumulator's last columns are read
-                        tc_fence_before();
-                        __syncwarp();
-                        if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
-                    }
+                    if (c + COLS >= PN / 2 || col0 + c + COLS >= p.n) release();
                     store_tile<T>(p, tile, row0, col0 + c, lane);
                 }
             } else {

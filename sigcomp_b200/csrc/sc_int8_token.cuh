@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
         uint32_t m = 0;
         if (live)
             for (int c = th * V::N; c < p.k; c += PER * 32 * V::N)
-                m = V::top(packed ? load_vec<E, true>(row, c, p.k) : load_vec<E, false>(row, c, p.k), m);
+                m = V::top(packed && c + V::N <= p.k ? *reinterpret_cast<const uint4 *>(row + c) : load_elements<E>(row + c, row, row + p.k), m);
         m = __reduce_max_sync(0xffffffffu, V::top_bits(m));
         if (lane == 0) tops[warp] = m;
         __syncthreads();
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
         for (int c = th * V::N; c < kpad; c += PER * 32 * V::N) {
             uint32_t o[V::N / 4] = {};
             if (live && rs.finite && c < p.k)
-                V::quantise(packed ? load_vec<E, true>(row, c, p.k) : load_vec<E, false>(row, c, p.k), rs.r, o);
+                V::quantise(packed && c + V::N <= p.k ? *reinterpret_cast<const uint4 *>(row + c) : load_elements<E>(row + c, row, row + p.k), rs.r, o);
 #pragma unroll
             for (int i = 0; i < V::N / 4; ++i) *reinterpret_cast<uint32_t *>(xq + t * kpad + c + 4 * i) = o[i];
         }

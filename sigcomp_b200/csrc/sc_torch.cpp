@@ -111,18 +111,24 @@ at::Tensor empty(c10::IntArrayRef sizes, c10::ScalarType type, const at::Tensor 
     return at::detail::empty_cuda(sizes, type, beside.device(), c10::nullopt);
 }
 
-// int8 of the given shape whose rows start a multiple of 16 bytes apart, as the matrix kernels read them
-at::Tensor empty_int8(c10::IntArrayRef lead, int64_t cols, const at::Tensor &beside)
+// elements from row to row of results: a multiple of 16 bytes, as the kernels read and write whole vectors
+int64_t padded(int64_t cols, c10::ScalarType type)
+{
+    const int64_t vec = 16 / (int64_t)c10::elementSize(type);
+    return (cols + vec - 1) / vec * vec;
+}
+
+at::Tensor empty_rows(c10::IntArrayRef lead, int64_t cols, c10::ScalarType type, const at::Tensor &beside)
 {
     c10::SmallVector<int64_t, 6> sizes(lead.begin(), lead.end()), strides(lead.size() + 1);
     sizes.push_back(cols);
-    int64_t step = (cols + 15) / 16 * 16;
+    int64_t step = padded(cols, type);
     strides[lead.size()] = 1;
     for (size_t i = lead.size(); i-- > 0;) {
         strides[i] = step;
         step *= lead[i] > 0 ? lead[i] : 1;
     }
-    return at::detail::empty_strided_cuda(sizes, strides, c10::ScalarType::Char, beside.device());
+    return at::detail::empty_strided_cuda(sizes, strides, type, beside.device());
 }
 
 void *stream_of(const at::Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -167,9 +173,9 @@ PyObject *quantize(PyObject *const *a)
     const at::Tensor &x = tensor("x", a[0], FLOATS);
     at::Tensor rows = as_rows("x", x);
     on_gpu(x);
-    at::Tensor q = empty_int8(leading(x), x.size(-1), x), s = empty(leading(x), c10::ScalarType::Float, x);
+    at::Tensor q = empty_rows(leading(x), x.size(-1), c10::ScalarType::Char, x), s = empty(leading(x), c10::ScalarType::Float, x);
     check(sc_quantize_tokens_device(x.device().index(), rows.data_ptr(), sc_type(x.scalar_type()), rows.size(0), rows.size(1),
-                                    row_stride(rows), (int8_t *)q.data_ptr(), (x.size(-1) + 15) / 16 * 16,
+                                    row_stride(rows), (int8_t *)q.data_ptr(), padded(x.size(-1), c10::ScalarType::Char),
                                     (float *)s.data_ptr(), stream_of(x)));
     return pair(std::move(q), std::move(s));
 }
@@ -187,10 +193,10 @@ PyObject *dequantize(PyObject *const *a)
         if (one == -1.0 && PyErr_Occurred()) return nullptr;
     }
     on_gpu(q);
-    at::Tensor y = empty(q.sizes(), type, q);
+    at::Tensor y = empty_rows(leading(q), q.size(-1), type, q);
     check(sc_dequantize_tokens_device(q.device().index(), (const int8_t *)rows.data_ptr(), row_stride(rows),
                                       scales.defined() ? (const float *)scales.data_ptr() : nullptr, (float)one, rows.size(0),
-                                      rows.size(1), y.data_ptr(), sc_type(type), rows.size(1), stream_of(q)));
+                                      rows.size(1), y.data_ptr(), sc_type(type), padded(q.size(-1), type), stream_of(q)));
     return THPVariable_Wrap(std::move(y));
 }
 
@@ -231,17 +237,9 @@ PyObject *linear(PyObject *const *a, bool int8_out)
     if (n > 1 && w.stride(0) < k) w = w.contiguous();       // rows that overlap, as those of an expanded row do
     const int64_t m = rows.size(0), x_stride = row_stride(rows), w_stride = row_stride(w);
     const int xt = sc_type(x.scalar_type()), yt = sc_type(type);
-    at::Tensor y, y_scales, work;
-    int64_t y_stride = n;
-    if (int8_out) {
-        y = empty_int8(leading(x), n, x);
-        y_stride = (n + 15) / 16 * 16;
-        if (row_out) y_scales = empty(leading(x), c10::ScalarType::Float, x);
-    } else {
-        c10::SmallVector<int64_t, 6> sizes(x.sizes().begin(), x.sizes().end());
-        sizes.back() = n;
-        y = empty(sizes, type, x);
-    }
+    at::Tensor y = empty_rows(leading(x), n, type, x), y_scales, work;
+    const int64_t y_stride = padded(n, type);
+    if (row_out) y_scales = empty(leading(x), c10::ScalarType::Float, x);
     const int x_packed = ((uintptr_t)rows.data_ptr() | (uintptr_t)x_stride) % 16 == 0 && x_stride >= k;
     const int w_packed = ((uintptr_t)w.data_ptr() | (uintptr_t)w_stride) % 16 == 0;
     const int64_t bytes = sc_int8_linear_workspace(xt, x_packed, w_packed, m, n, k, yt, row_out);

@@ -15,7 +15,9 @@ whole numbers, exact in 32 bits, and the roundings after them are fixed (include
 writes them out).  So teacher-forced coding in large batches and decoding token by token agree bit
 for bit.
 
-Arrays are torch tensors on one GPU; leading dimensions are batch dimensions.  Work is put into the
+Arrays are torch tensors on one GPU; leading dimensions are batch dimensions.  Rows of every result
+start a multiple of 16 bytes apart, so results are contiguous where their width is such a multiple, and
+strided otherwise (rows of odd widths side by side took two to five times as long to write).  Work is put into the
 current stream of that GPU and not waited for, so calls can be captured into CUDA graphs.  The
 operators serve coding, not training: a tensor that asks for a gradient is refused.
 """
@@ -40,7 +42,6 @@ def quantize_tokens(x):
     ``a = max(max|row|, 2**-100)``, ``scale = a / 127`` and ``q = rint(row * (127 / a))``; both
     quotients are rounded to float32, the product is not, and ties go to the even number.  A row
     holding an infinity or a NaN gets the scale NaN and zeros, so what is computed from it is NaN.
-    Rows of ``q`` start a multiple of 16 bytes apart.
     """
     return _int8.quantize_tokens(x)
 

@@ -191,7 +191,7 @@ def test_linear(ops, rows, k, n, dtype):
     relu, bias = (rows + n) % 2 == 1, (rows + k) % 3 != 0
     w, ws, b = layer(n, k, n, bias)
     y = ops.int8_linear(q, w, ws, b, x_scales=s, relu=relu, dtype=dtype)
-    assert y.dtype == dtype and y.is_contiguous()
+    assert y.dtype == dtype and y.stride(0) * y.element_size() % 16 == 0
     same(y, want_linear(host(q), host(s), host(w), host(ws), host(b), relu))
 
 
@@ -394,3 +394,60 @@ def test_entropy_model_of_int8_layers_codes_and_decodes(ops):
                                                   streams, p(back), None, st))
     assert np.array_equal(back.cpu().numpy().reshape(streams, steps), symbols)
     codec.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(5, 3), (300, 8), (1000, 21), (700, 130), (33, 1023), (9, 4099), (4, 16383)])
+@pytest.mark.parametrize("shift", [0, 1, 2, 5])
+def test_rows_at_any_address(ops, dtype, rows, cols, shift):
+    """Rows of x, of q and of the values that start at any element, read and written whole: nothing before the
+    first row, between rows or behind the last one is touched."""
+    x = float_rows(rows, cols, dtype, rows + shift)
+    flat = torch.full((rows * cols + 40,), float("nan"), dtype=dtype, device=DEV)
+    view = flat[shift:shift + rows * cols].view(rows, cols)
+    view.copy_(x)
+    q, s = ops.quantize_tokens(view)
+    wq, ws = want_quantized(host(x))
+    same(q, wq)
+    same(s, ws)
+    # q and the values in buffers with a rim of their own, rows close together
+    L, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    rim = torch.full((rows * cols + 40,), 77, dtype=torch.int8, device=DEV)
+    _lib.check(L.sc_quantize_tokens_device(0, view.data_ptr(), code, rows, cols, cols, rim.data_ptr() + shift, cols,
+                                           s.data_ptr(), st))
+    same(rim[shift:shift + rows * cols].view(rows, cols), wq)
+    assert (rim[:shift] == 77).all() and (rim[shift + rows * cols:] == 77).all()
+    out = torch.full((rows * cols + 40,), 5.0, dtype=dtype, device=DEV)
+    for q_at, q_stride in ((q.data_ptr(), q.stride(0)), (rim.data_ptr() + shift, cols)):
+        out.fill_(5.0)
+        _lib.check(L.sc_dequantize_tokens_device(0, q_at, q_stride, s.data_ptr(), 0.0, rows, cols,
+                                                 out.data_ptr() + shift * out.element_size(), code, cols, st))
+        with np.errstate(over="ignore"):
+            same(out[shift:shift + rows * cols].view(rows, cols),
+                 torch.from_numpy(wq.astype(np.float32) * ws[:, None]).to(dtype).float().numpy())
+        assert (out[:shift] == 5).all() and (out[shift + rows * cols:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16, torch.int8])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 33), (20, 96, 129), (700, 64, 259), (20000, 64, 131), (20001, 40, 10)])
+@pytest.mark.parametrize("shift,gap", [(0, 0), (1, 0), (3, 5)])
+def test_results_at_any_address(ops, dtype, rows, k, n, shift, gap):
+    """Results in rows that start at any element and have a gap between them, which stays."""
+    q, s = int8_rows(rows, k, 4), scales_of(rows, 5)
+    w, ws, b = layer(n, k, 6)
+    out = torch.full((shift + rows * (n + gap) + 9,), 5, dtype=dtype, device=DEV)
+    L = _lib.load()
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3}[dtype]
+    size = L.sc_int8_linear_workspace(3, 1, 1, rows, n, k, code, 0)
+    work = torch.empty(max(size, 1), dtype=torch.uint8, device=DEV)
+    _lib.check(L.sc_int8_linear_device(0, q.data_ptr(), 3, q.stride(0) if rows > 1 else -(-k // 16) * 16, s.data_ptr(),
+                                       w.data_ptr(), w.stride(0), ws.data_ptr(), b.data_ptr(), rows, n, k, 1,
+                                       out.data_ptr() + shift * out.element_size(), code, n + gap, None, 0.02,
+                                       work.data_ptr() if size else None, size, torch.cuda.current_stream().cuda_stream))
+    want = want_linear(host(q), host(s), host(w), host(ws), host(b), True)
+    if dtype == torch.int8:
+        want = np.clip(np.rint(want / np.float32(0.02)), -128, 127)
+    got = out[shift:shift + rows * (n + gap)].view(rows, n + gap)
+    same(got[:, :n], want)
+    assert (got[:, n:] == 5).all() and (out[:shift] == 5).all() and (out[shift + rows * (n + gap):] == 5).all()
