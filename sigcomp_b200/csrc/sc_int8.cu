@@ -338,30 +338,27 @@ k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__rest
             if (r >= rows) continue;
             const int8_t *qr = q + r * q_stride;
             s[u] = scales ? scales[r] : scale;
-            if (ALIGNED) {
-                if (c[u] + N <= cols) {
-                    if constexpr (N == 8) {
-                        const uint2 v = *reinterpret_cast<const uint2 *>(qr + c[u]);
-                        raw[u][0] = v.x, raw[u][N / 4 - 1] = v.y;
-                    } else raw[u][0] = *reinterpret_cast<const uint32_t *>(qr + c[u]);
-                }
-            } else {
-                c[u] -= (int)(((uintptr_t)(y + r * y_stride) & 15) / sizeof(T));
+            if (!ALIGNED) c[u] -= (int)(((uintptr_t)(y + r * y_stride) & 15) / sizeof(T));
+            const bool whole = c[u] >= 0 && c[u] + N <= cols;
+            if (ALIGNED && whole) {
+                if constexpr (N == 8) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(qr + c[u]);
+                    raw[u][0] = v.x, raw[u][N / 4 - 1] = v.y;
+                } else raw[u][0] = *reinterpret_cast<const uint32_t *>(qr + c[u]);
+            } else if (!ALIGNED && q_words && whole && (r + 1 < rows || c[u] + N + 4 <= cols)) {
                 // the words may reach four bytes behind the vector, which lie in q but at its very end
-                if (q_words && c[u] >= 0 && c[u] + N <= cols && (r + 1 < rows || c[u] + N + 4 <= cols)) {
-                    const uint32_t *at = reinterpret_cast<const uint32_t *>(qr + (c[u] & ~3));
-                    uint32_t w[N / 4 + 1];
+                const uint32_t *at = reinterpret_cast<const uint32_t *>(qr + (c[u] & ~3));
+                uint32_t w[N / 4 + 1];
 #pragma unroll
-                    for (int i = 0; i <= N / 4; ++i) w[i] = at[i];
+                for (int i = 0; i <= N / 4; ++i) w[i] = at[i];
 #pragma unroll
-                    for (int i = 0; i < N / 4; ++i) raw[u][i] = __funnelshift_r(w[i], w[i + 1], (c[u] & 3) * 8);
-                } else {
+                for (int i = 0; i < N / 4; ++i) raw[u][i] = __funnelshift_r(w[i], w[i + 1], (c[u] & 3) * 8);
+            } else {
+                uint32_t b[N];
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        if (i % 4 == 0) raw[u][i / 4] = 0;
-                        if (c[u] + i >= 0 && c[u] + i < cols) raw[u][i / 4] |= (uint32_t)(uint8_t)qr[c[u] + i] << (8 * (i % 4));
-                    }
-                }
+                for (int i = 0; i < N; ++i) b[i] = c[u] + i >= 0 && c[u] + i < cols ? (uint32_t)(uint8_t)qr[c[u] + i] : 0;
+#pragma unroll
+                for (int i = 0; i < N / 4; ++i) raw[u][i] = pack4(b[4 * i], b[4 * i + 1], b[4 * i + 2], b[4 * i + 3]);
             }
         }
 #pragma unroll
@@ -369,16 +366,11 @@ k_dequantize(const int8_t *__restrict__ q, int64_t q_stride, const float *__rest
             const int64_t r = row0 + u * deep;
             if (r >= rows) continue;
             T *yr = y + r * y_stride;
-            if (ALIGNED && c[u] + N > cols) {
-                for (int i = 0; i < N && c[u] + i < cols; ++i)
-                    yr[c[u] + i] = from_f32<T>(__fmul_rn((float)q[r * q_stride + c[u] + i], s[u]));
-                continue;
-            }
             __align__(16) T out[N];
 #pragma unroll
             for (int i = 0; i < N; ++i)
                 out[i] = from_f32<T>(__fmul_rn((float)(int8_t)(raw[u][i / 4] >> (8 * (i % 4))), s[u]));
-            if (ALIGNED || (c[u] >= 0 && c[u] + N <= cols)) {
+            if (c[u] >= 0 && c[u] + N <= cols) {
                 *reinterpret_cast<uint4 *>(yr + c[u]) = *reinterpret_cast<const uint4 *>(out);
             } else {
 #pragma unroll

@@ -430,8 +430,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                     const int ab = (uu + h) & 1;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], ((uu + h) >> 1) & 1)))) break;
                     tc_fence_after();
+                    const int live = p.n - h * PN - grp * (PN / 2);            // channels of this warp's half
 #pragma unroll 1
-                    for (int c = 0; c < PN / 2; c += 32) {
+                    for (int c = 0; c < PN / 2 && c < live; c += 32) {
                         uint32_t v[2][16];
                         tmem_ld_16x32(lane_base + ab * PN + c, v[0]);
                         tmem_ld_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
@@ -471,15 +472,10 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 const float least = p.relu ? kMagic : -INFINITY;
                 for (int h = 0; h < nu; ++h) {
                     const int ab = (uu + h) & 1;
-                    uint32_t v[2][32];                         // the next columns are on their way meanwhile
-                    tmem_ld32(lane_base + ab * PN, v[0]);
+                    const int live = p.n - h * PN - grp * (PN / 2);
                     staging_free(p, lane);
-#pragma unroll
-                    for (int c = 0; c < PN / 2; c += 32) {
-                        const uint32_t(&now)[32] = v[c / 32 % 2];
+                    auto scale32 = [&](const uint32_t(&now)[32], int c) {
                         uint32_t o[8];
-                        tmem_ld_wait();
-                        if (c + 32 < PN / 2) tmem_ld32(lane_base + ab * PN + c + 32, v[(c / 32 + 1) % 2]);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             F2 z[2];
@@ -500,6 +496,24 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16)) = make_uint4(o[0], o[1], o[2], o[3]);
                         *reinterpret_cast<uint4 *>(tile + sw128_offset(lane, c / 16 + 1)) =
                             make_uint4(o[4], o[5], o[6], o[7]);
+                    };
+                    if (live >= PN / 2) {
+                        uint32_t v[2][32];                     // the next columns are on their way meanwhile
+                        tmem_ld32(lane_base + ab * PN, v[0]);
+#pragma unroll
+                        for (int c = 0; c < PN / 2; c += 32) {
+                            tmem_ld_wait();
+                            if (c + 32 < PN / 2) tmem_ld32(lane_base + ab * PN + c + 32, v[(c / 32 + 1) % 2]);
+                            scale32(v[c / 32 % 2], c);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < live; c += 32) {
+                            uint32_t v[32];
+                            tmem_ld32(lane_base + ab * PN + c, v);
+                            tmem_ld_wait();
+                            scale32(v, c);
+                        }
                     }
                     tc_fence_before();
                     __syncwarp();
