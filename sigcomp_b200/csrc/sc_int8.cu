@@ -560,8 +560,12 @@ void dequantize(const int8_t *q, int64_t qs, const float *scales, float scale, i
     constexpr int N = Vec<T>::N;
     const bool al = aligned(q, qs, N) && aligned(y, ys * (int64_t)sizeof(T), 16);
     const int wide_cols = al ? cols : cols + N - 1;             // a row's vectors may begin before it
+    // as wide as a row, or of the widths from a warp's up the one that leaves the fewest lanes behind its end
     int log_lanes = 0;
     while (log_lanes < 8 && (N << log_lanes) < wide_cols) ++log_lanes;
+    auto behind = [&](int l) { return ((int64_t)wide_cols + (N << l) - 1) / (N << l) * (N << l); };
+    for (int l = log_lanes - 1; l >= 5; --l)
+        if (behind(l) < behind(log_lanes)) log_lanes = l;
     const int64_t deep = (256 >> log_lanes) * 4, wide = (int64_t)N << log_lanes;
     const dim3 g(grid_x((rows + deep - 1) / deep), (unsigned)std::min<int64_t>((wide_cols + wide - 1) / wide, 65535));
     if (al) launch(k_dequantize<T, true>, g, 256, 0, s, 1, q, qs, scales, scale, rows, cols, y, ys, log_lanes, 1);
@@ -596,7 +600,8 @@ template <> constexpr CUtensorMapDataType map_type<int8_t>() { return CU_TENSOR_
 
 // y (T; int8: requantised with a scale for each row, at most 512 channels) of int8 rows, on SM pairs
 template <typename T, int MODE>
-void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, cudaStream_t s)
+void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y, int64_t y_stride, cudaStream_t s,
+                   uint32_t *tops = nullptr)
 {
     static std::atomic<uint64_t> ready{0};
     allow_smem(k_pair<T, MODE>, P_SMEM, ready);
@@ -616,6 +621,7 @@ void product_pairs(const Int8Linear &p, Rows8 x, const float *xs, Rows8 w, T *y,
     a.y_stride = y_stride;
     a.y_scales = p.y_scales;
     a.output_scale = p.output_scale;
+    a.tops = tops;
     const int64_t tiles = (p.rows + 2 * PM - 1) / (2 * PM), units = (p.n + PN - 1) / PN;
     const int64_t work = MODE == ROWS ? tiles : tiles * units;
     const unsigned pairs = (unsigned)std::min<int64_t>(work, sm_count() / 2);
@@ -708,7 +714,7 @@ int cluster_room(int ctas)
 // What multiplies a number of rows: the kernel, its tile and split, whether the rows are quantised by a launch of
 // their own, and the time in microseconds that it is expected to take.
 struct Way {
-    enum { TOKEN, FEW, FEW_ROWS, PAIRS, PAIRS_ROWS } kernel;
+    enum { TOKEN, FEW, FEW_ROWS, PAIRS, PAIRS_ROWS, PAIRS_TWICE } kernel;
     int bt, split;
     TokenPlan t;
     bool requant;
@@ -751,12 +757,16 @@ Way choose(int64_t rows, int64_t n, int64_t k, bool rows_out)
                 offer(Way::FEW_ROWS, 16, split, false, 3.2 + 0.24 * (double)((nkb + split - 1) / split));
         if (blocks <= 2)
             offer(Way::PAIRS_ROWS, 0, 1, false, 4.2 + waves(tiles, pairs) * ((double)blocks * 0.3 * (double)nkb + 2.9));
+        // both launches multiply; nothing in 32 bits leaves the chip (28,467 rows of 128 x 4,650: 156 us against 292,
+        // 20,480 of 1,024 x 1,024: 42 against 54)
+        offer(Way::PAIRS_TWICE, 0, 1, false,
+              10.0 + waves(tiles * blocks, pairs) * (2 * std::max(0.3 * (double)nkb, 0.2) + 2.6));
     }
     return best;
 }
 
 // The rows of a call, cut in two where the pair kernel's last wave would leave most SMs idle for the time that its
-// K takes: 20,480 rows of 8,192 x 512 requantised, 97 us in two waves, TODO us as one wave and 1,536 rows apart.
+// K takes: 20,480 rows of 8,192 x 512 requantised, 97 us in two waves, 82 us as one wave and 1,536 rows apart.
 struct Ways {
     int64_t cut;                 // rows of the first way; the others take the second
     Way way[2];
@@ -802,7 +812,7 @@ static int64_t pad(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 struct Plan {
     Ways ways;
     bool quantise, spread_x, spread_w;
-    int64_t wide;                // rows of the product in 32 bits
+    int64_t wide;                // bytes of the product in 32 bits, or of the rows' largest magnitudes
     int64_t bytes;
 };
 
@@ -815,12 +825,15 @@ static Plan plan(const Int8Linear &p)
     o.quantise = p.x_type != SC_TYPE_I8 && !token;
     o.spread_x = p.x_type == SC_TYPE_I8 && !token && !p.x_packed;
     o.spread_w = !p.w_packed;
-    o.wide = w[0].requant ? o.ways.cut : 0;
-    if (o.ways.cut < p.rows && w[1].requant) o.wide = std::max(o.wide, p.rows - o.ways.cut);
+    auto wide = [&](const Way &way, int64_t rows) {
+        return way.requant ? rows * pad(p.n, 4) * 4 : way.kernel == Way::PAIRS_TWICE ? rows * 4 : 0;
+    };
+    o.wide = wide(w[0], o.ways.cut);
+    if (o.ways.cut < p.rows) o.wide = std::max(o.wide, wide(w[1], p.rows - o.ways.cut));
     if (o.quantise) o.bytes += pad(p.rows * 4, 256);
     if (o.quantise || o.spread_x) o.bytes += pad(p.rows * pad(p.k, 16), 256);
     if (o.spread_w) o.bytes += pad(p.n * pad(p.k, 16), 256);
-    o.bytes += pad(o.wide * pad(p.n, 4) * 4, 256);
+    o.bytes += pad(o.wide, 256);
     return o;
 }
 
@@ -850,6 +863,13 @@ static void multiply(const Int8Linear &p, const Way &way, Rows8 x, const float *
         break;
     case Way::FEW_ROWS: launch_few<16, true>(p, x, xs, w, (int8_t *)y, ys, way.split, s); break;
     case Way::PAIRS_ROWS: product_pairs<int8_t, ROWS>(p, x, xs, w, (int8_t *)y, ys, s); break;
+    case Way::PAIRS_TWICE: {
+        uint32_t *tops = (uint32_t *)wide;
+        SC_CUDA(cudaMemsetAsync(tops, 0, (size_t)p.rows * 4, s));
+        product_pairs<int8_t, TOPS>(p, x, xs, w, (int8_t *)y, ys, s, tops);
+        product_pairs<int8_t, BY_TOPS>(p, x, xs, w, (int8_t *)y, ys, s, tops);
+        break;
+    }
     case Way::PAIRS:
         if (y_type == SC_TYPE_I8) product_pairs<int8_t, STATIC>(p, x, xs, w, (int8_t *)y, ys, s);
         else if (y_type == SC_TYPE_F32) product_pairs<float, PLAIN>(p, x, xs, w, (float *)y, ys, s);
@@ -887,20 +907,21 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
     }
     if (o.spread_w) w = spread(p.w, p.n, p.w_stride);
     float *wide = (float *)ws;
-    Int8Linear part = p;
-    part.rows = o.ways.cut;
-    multiply(part, o.ways.way[0], x, xs, w, wide, s);
-    if (o.ways.cut < p.rows) {
-        const int64_t cut = o.ways.cut, e = p.y_type == SC_TYPE_F32 ? 4 : p.y_type == SC_TYPE_I8 ? 1 : 2;
-        part.rows = p.rows - cut;
-        part.y = (uint8_t *)p.y + cut * p.y_stride * e;
-        part.y_scales = p.y_scales ? p.y_scales + cut : nullptr;
-        // never k_token on a float x: the rest has more than two rows, or x is int8 by now
-        part.x = x.p + cut * x.stride;
-        part.x_type = SC_TYPE_I8;
-        part.x_stride = x.stride;
-        multiply(part, o.ways.way[1], {x.p + cut * x.stride, x.stride}, xs + cut, w, wide, s);
-    }
+    // rows r .. r + count on their way
+    auto rows_of = [&](int64_t r, int64_t count, const Way &way) {
+        Int8Linear part = p;
+        part.rows = count;
+        part.y = (uint8_t *)p.y + r * p.y_stride * (p.y_type == SC_TYPE_F32 ? 4 : p.y_type == SC_TYPE_I8 ? 1 : 2);
+        part.y_scales = p.y_scales ? p.y_scales + r : nullptr;
+        if (r > 0) {            // x is int8 here: k_token takes a float x whole
+            part.x = x.p + r * x.stride;
+            part.x_type = SC_TYPE_I8;
+            part.x_stride = x.stride;
+        }
+        multiply(part, way, {x.p + r * x.stride, x.stride}, xs ? xs + r : nullptr, w, wide, s);
+    };
+    rows_of(0, o.ways.cut, o.ways.way[0]);
+    if (o.ways.cut < p.rows) rows_of(o.ways.cut, p.rows - o.ways.cut, o.ways.way[1]);
 }
 
 int int8_device_error()

@@ -26,6 +26,9 @@ using namespace tc;
 // pass over half 0 runs under the products of half 1, the second over half 1 under those of the next
 // tile's half 0.
 //
+// Rows of more channels are quantised by two launches that both multiply: the first keeps the rows' largest magnitudes
+// (TOPS), the second quantises by them (BY_TOPS).
+//
 // Every wait is bounded; a warp that gives up ends, and the others end on their own limits.
 constexpr int PM = 128;                        // rows per CTA
 constexpr int PN = 256;                        // channels per unit
@@ -45,8 +48,9 @@ constexpr int P_OFF_TMEM = P_OFF_CNT + P_EPI * 4;
 constexpr int P_SMEM = P_OFF_TMEM + 16 + 1024;                     // + alignment slack
 static_assert(P_SMEM <= 232448, "shared memory per CTA");
 
-// what becomes of the results in 32 bits: rounded to T, quantised row by row, or by one scale
-enum { PLAIN, ROWS, STATIC };
+// What becomes of the results in 32 bits: rounded to T; quantised row by row; by one scale; only their rows' largest
+// magnitudes kept; quantised by those.
+enum { PLAIN, ROWS, STATIC, TOPS, BY_TOPS };
 
 struct PairParams {
     CUtensorMap x, w;                          // box 128 rows x 128 bytes
@@ -59,6 +63,7 @@ struct PairParams {
     int64_t y_stride;
     float *y_scales;
     float output_scale;
+    uint32_t *tops;                            // TOPS, BY_TOPS: bits of the rows' largest magnitudes
 };
 
 // One lane of a converged warp, the same each time.  The loops around TMA and MMA are run by whole warps
@@ -376,7 +381,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 }
                 __syncwarp();
             }
-            if constexpr (!REQUANT) {
+            if constexpr (MODE == PLAIN || MODE == STATIC) {
                 const int ab = uu & 1;
                 const int col0 = block * PN + grp * (PN / 2);
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], (uu >> 1) & 1)))) break;
@@ -426,11 +431,12 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 // with ReLU the row's largest result, or 0, is its largest magnitude; the results themselves
                 // stay as they are until they are scaled
                 float top[4] = {};
-                for (int h = 0; h < nu && ok; ++h) {
+                const int halves = REQUANT ? nu : 1, first_block = REQUANT ? 0 : block;
+                for (int h = 0; h < halves && ok; ++h) {
                     const int ab = (uu + h) & 1;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], ((uu + h) >> 1) & 1)))) break;
                     tc_fence_after();
-                    const int live = p.n - h * PN - grp * (PN / 2);            // channels of this warp's half
+                    const int live = p.n - (first_block + h) * PN - grp * (PN / 2);            // channels of this warp's half
 #pragma unroll 1
                     for (int c = 0; c < PN / 2 && c < live; c += 32) {
                         uint32_t v[2][16];
@@ -438,41 +444,64 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         tmem_ld_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
                         tmem_ld_wait();
                         affine_16x32(v, reinterpret_cast<const float4 *>(tb + h * PN) + c / 2 + cl, s);
-                        tmem_st_16x32(lane_base + ab * PN + c, v[0]);
-                        tmem_st_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
+                        if (MODE != TOPS) {
+                            tmem_st_16x32(lane_base + ab * PN + c, v[0]);
+                            tmem_st_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
+                        }
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
+                            for (int i = 0; i < 4 && MODE != BY_TOPS; ++i) {
                                 const float y0 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2)]);
                                 const float y1 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2) + 1]);
                                 top[i] = p.relu ? max3_nan(top[i], y0, y1) : max3_abs_nan(top[i], y0, y1);
                             }
                     }
-                    tmem_st_wait();
+                    if (MODE != TOPS) tmem_st_wait();
                 }
                 if (!ok) break;
-                // the row's other half of the columns is with the other warp of this quarter, which
-                // cannot be more than one tile ahead: two parities of the buffer are enough
-                float *mx = row_max + (step & 1) * 2 * PM;
+                if constexpr (MODE == TOPS) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[uu & 1], 0));
+                    ++uu;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                    top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                    if (cl == i) mx[grp * PM + q * 32 + rl + 8 * i] = top[i];
+                    for (int i = 0; i < 4; ++i) {
+                        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                        // magnitudes' bits are in their order, whichever comes first
+                        const int64_t row = row0 + rl + 8 * i;
+                        if (cl == i && row < p.rows) atomicMax(p.tops + row, magnitude(top[i]));
+                    }
+                    continue;
                 }
-                __syncwarp();
-                if (elect_one()) counter_add_release(&max_cnt[grp * 4 + q], 1);
-                if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], step + 1)))) break;
-                // from here on a thread has a row of its own: its results lie in 16 bytes at a time
                 const int mine = q * 32 + lane;
-                const RowScale rs = row_scale(magnitude(max_nan(mx[mine], mx[PM + mine])));
-                if (grp == 0 && row0 + lane < p.rows) p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                uint32_t largest = 0;
+                if constexpr (MODE == BY_TOPS) {
+                    if (row0 + lane < p.rows) largest = p.tops[row0 + lane];
+                } else {
+                    // the row's other half of the columns is with the other warp of this quarter, which
+                    // cannot be more than one tile ahead: two parities of the buffer are enough
+                    float *mx = row_max + (step & 1) * 2 * PM;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                        if (cl == i) mx[grp * PM + q * 32 + rl + 8 * i] = top[i];
+                    }
+                    __syncwarp();
+                    if (elect_one()) counter_add_release(&max_cnt[grp * 4 + q], 1);
+                    if (!(ok = __all_sync(0xffffffffu, counter_wait(&max_cnt[(grp ^ 1) * 4 + q], step + 1)))) break;
+                    largest = magnitude(max_nan(mx[mine], mx[PM + mine]));
+                }
+                // from here on a thread has a row of its own: its results lie in 16 bytes at a time
+                const RowScale rs = row_scale(largest);
+                if (grp == 0 && first_block == 0 && row0 + lane < p.rows) p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
                 const bool all_finite = __all_sync(0xffffffffu, rs.finite);
                 const float least = p.relu ? kMagic : -INFINITY;
-                for (int h = 0; h < nu; ++h) {
+                for (int h = 0; h < halves; ++h) {
                     const int ab = (uu + h) & 1;
-                    const int live = p.n - h * PN - grp * (PN / 2);
+                    const int live = p.n - (first_block + h) * PN - grp * (PN / 2);
                     staging_free(p, lane);
                     auto scale32 = [&](const uint32_t(&now)[32], int c) {
                         uint32_t o[8];
@@ -518,9 +547,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                     tc_fence_before();
                     __syncwarp();
                     if (elect_one()) mbar_arrive_cluster_relaxed(map_to_rank(&acc_empty[ab], 0));
-                    store_tile<int8_t>(p, tile, row0, h * PN + grp * (PN / 2), lane);
+                    store_tile<int8_t>(p, tile, row0, (first_block + h) * PN + grp * (PN / 2), lane);
                 }
-                uu += nu;
+                uu += halves;
             }
         }
         if (p.y_tma && elect_one()) bulk_wait_all();

@@ -181,7 +181,7 @@ SIZES = [(1, 1, 1), (1, 64, 512), (1, 8192, 512), (1, 4097, 130), (2, 17, 3), (3
          (8, 8192, 96), (9, 96, 257), (16, 512, 512), (17, 4096, 640), (31, 129, 100), (64, 8192, 512), (65, 512, 256),
          (100, 300, 1100), (127, 128, 128), (128, 128, 256), (129, 1, 257), (200, 2048, 64), (255, 511, 511),
          (257, 129, 513), (300, 1000, 777), (640, 512, 512), (1001, 96, 2304), (2049, 640, 300), (5000, 512, 256),
-         (20000, 64, 16), (40000, 128, 512)]
+         (20000, 64, 16), (40000, 128, 512), (9001, 64, 1300), (20000, 300, 700), (30011, 48, 2049)]
 
 
 @pytest.mark.parametrize("rows,k,n", SIZES)
