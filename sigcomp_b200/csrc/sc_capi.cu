@@ -153,6 +153,13 @@ bool rows_ok(int64_t rows, int64_t cols, int64_t stride)
     return rows >= 0 && rows < (1ll << 31) - 1024 && cols >= 1 && cols <= (1ll << 30) && stride >= cols;
 }
 
+// an array of SC_TYPE_* elements starts on one
+bool on_element(const void *p, int32_t type)
+{
+    const uintptr_t size = type == SC_TYPE_F32 ? 4 : type == SC_TYPE_I8 ? 1 : 2;
+    return (uintptr_t)p % size == 0;
+}
+
 int first_error(const uint8_t *errs, int64_t n)
 {
     for (int64_t c = 0; c < n; ++c)
@@ -773,7 +780,7 @@ int sc_quantize_tokens_device(int device, const void *x, int32_t x_type, int64_t
 {
     g_err[0] = 0;
     if (x_type < SC_TYPE_F32 || x_type > SC_TYPE_BF16 || !rows_ok(rows, cols, q_stride) || x_stride < 0 ||
-        (rows > 0 && (!x || !q || !scales))) {
+        (rows > 0 && (!x || !q || !scales)) || !on_element(x, x_type) || !on_element(scales, SC_TYPE_F32)) {
         set_error("invalid argument");
         return SC_ERR_INVALID_ARGUMENT;
     }
@@ -789,7 +796,7 @@ int sc_dequantize_tokens_device(int device, const int8_t *q, int64_t q_stride, c
 {
     g_err[0] = 0;
     if (y_type < SC_TYPE_F32 || y_type > SC_TYPE_BF16 || !rows_ok(rows, cols, y_stride) || q_stride < 0 ||
-        (rows > 0 && (!q || !y))) {
+        (rows > 0 && (!q || !y)) || !on_element(y, y_type) || !on_element(scales, SC_TYPE_F32)) {
         set_error("invalid argument");
         return SC_ERR_INVALID_ARGUMENT;
     }
@@ -824,7 +831,9 @@ int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_s
     g_err[0] = 0;
     if (x_type < SC_TYPE_F32 || x_type > SC_TYPE_I8 || y_type < SC_TYPE_F32 || y_type > SC_TYPE_I8 ||
         k > SC_INT8_MAX_K || !rows_ok(rows, n, y_stride) || !rows_ok(n, k, w_stride) || x_stride < 0 || !w ||
-        !w_scales || (rows > 0 && (!x || !y)) || (rows > 0 && (x_type == SC_TYPE_I8) != (x_scales != nullptr))) {
+        !w_scales || (rows > 0 && (!x || !y)) || (rows > 0 && (x_type == SC_TYPE_I8) != (x_scales != nullptr)) || !on_element(x, x_type) || !on_element(y, y_type) ||
+        !on_element(x_scales, SC_TYPE_F32) || !on_element(w_scales, SC_TYPE_F32) || !on_element(bias, SC_TYPE_F32) ||
+        !on_element(y_scales, SC_TYPE_F32)) {
         set_error("invalid argument");
         return SC_ERR_INVALID_ARGUMENT;
     }

@@ -509,13 +509,12 @@ constexpr int kSms = 148;
 
 int sm_count()
 {
-    static int counts[64];
-    int dev = 0;
+    static std::atomic<int> counts[64];
+    int dev = 0, n = 0;
     SC_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && counts[dev] > 0) return counts[dev];
-    int n = 0;
+    if (dev < 64 && (n = counts[dev].load(std::memory_order_relaxed)) > 0) return n;
     SC_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    if (dev < 64) counts[dev] = n;
+    if (dev < 64) counts[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
@@ -546,6 +545,7 @@ void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t
     else if (vecs <= 128 && !few) launch_quantize<T, 32, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128) launch_quantize<T, 128, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 512 && !few) launch_quantize<T, 128, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 256 && few) launch_quantize<T, 256, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024 && few) launch_quantize<T, 1024, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024) launch_quantize<T, 256, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 2048) launch_quantize<T, 512, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
@@ -745,7 +745,7 @@ Way choose(int64_t rows, int64_t n, int64_t k, bool rows_out)
     const struct { int bt; double fixed, block; } sizes[] = {{16, 2.9, 0.24}, {32, 3.4, 0.25}, {64, 4.3, 0.27}, {128, 6.1, 0.33}};
     for (const auto &z : sizes) {
         const int64_t count = (rows + z.bt - 1) / z.bt * channels;
-        if (count > 4 * kSms || rows <= 2 || (z.bt > 16 && rows <= z.bt / 2)) continue;
+        if (count > 4 * kSms || t.per_cta > 0 || (z.bt > 16 && rows <= z.bt / 2)) continue;
         for (int split = 1; split <= F_MAX_SPLIT && split <= nkb; split *= 2)
             offer(Way::FEW, z.bt, split, rows_out,
                   waves(count, cluster_room(split)) * (z.fixed + z.block * (double)((nkb + split - 1) / split)) + extra);

@@ -62,7 +62,7 @@ const at::Tensor &tensor(const char *name, PyObject *o, int types, const at::Ten
     const at::Tensor &t = THPVariable_Unpack(o);
     const int type = sc_type(t.scalar_type());
     if (type < 0 || !(types >> type & 1)) refuse("%s must be of type %s, not %s", name, type_names(types), c10::toString(t.scalar_type()));
-    if (t.layout() != c10::kStrided) refuse("%s must be a dense tensor", name);
+    if (t.layout() != c10::kStrided || t.is_neg()) refuse("%s must be a dense tensor, not a lazily negated one", name);
     if (beside && t.device() != beside->device())
         refuse("%s is on %s, the other arrays are on %s", name, t.device().str().c_str(), beside->device().str().c_str());
     if (t.requires_grad() && c10::GradMode::is_enabled())

@@ -451,3 +451,57 @@ def test_results_at_any_address(ops, dtype, rows, k, n, shift, gap):
     got = out[shift:shift + rows * (n + gap)].view(rows, n + gap)
     same(got[:, :n], want)
     assert (got[:, n:] == 5).all() and (out[:shift] == 5).all() and (out[shift + rows * (n + gap):] == 5).all()
+
+
+def test_wide_rows_in_a_graph(ops):
+    """More channels than two accumulators hold: both launches that multiply, captured and replayed."""
+    x, layers = int8_rows(6000, 96, 1), layer(1300, 96, 2)
+    s = scales_of(6000, 3)
+    want = ops.int8_linear_requant(x, s, *layers, relu=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.int8_linear_requant(x, s, *layers, relu=True)
+    for _ in range(3):
+        got[0].zero_()
+        got[1].zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_calls_from_several_threads(ops):
+    """Calls of several host threads, each on a stream of its own, at the same time."""
+    from concurrent.futures import ThreadPoolExecutor
+    layers = [layer(512, 1024, 1), layer(900, 512, 2), layer(300, 900, 3)]
+    xs = [float_rows(rows, 1024, torch.float16, rows) for rows in (1, 3, 40, 700, 3000)]
+    want = [_chain(ops, x, layers, 0.02).clone() for x in xs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            out = [_chain(ops, xs[i], layers, 0.02) for _ in range(20)]
+        st.synchronize()
+        return all(torch.equal(o, want[i]) for o in out)
+
+    with ThreadPoolExecutor(5) as pool:
+        assert all(pool.map(work, range(5)))
+
+
+def test_weights_written_right_before_the_call(ops):
+    """The launch before a call writes what the call reads: weights, scales and tokens."""
+    for rows in (1, 20, 3000):
+        for seed in range(6):
+            wf = float_rows(512, 768, torch.bfloat16, seed)
+            x = float_rows(rows, 768, torch.bfloat16, seed + 50)
+            w, ws = ops.quantize_tokens(wf)
+            y = ops.int8_linear(x, w, ws)
+            wq, wscale = want_quantized(host(wf))
+            q, s = want_quantized(host(x))
+            same(y, torch.from_numpy(want_linear(q, s, wq, wscale, None, False)).to(torch.bfloat16).float().numpy())
+
+
+def test_no_wait_has_timed_out(ops):
+    ops.check_waits(DEV)
+    ops.check_waits()

@@ -1,7 +1,5 @@
 """Refusals of the int8 operators and of their C entry points, which need no GPU."""
 
-import ctypes
-
 import pytest
 import torch
 
@@ -35,6 +33,8 @@ def test_arrays_off_the_gpu_are_refused():
     ("at least one element", lambda: quantize_tokens(torch.zeros((3, 0)))),
     ("at least one element", lambda: quantize_tokens(torch.tensor(1.0))),
     ("gradient", lambda: quantize_tokens(X.clone().requires_grad_())),
+    ("dense", lambda: quantize_tokens(torch.zeros(3, 4).to_sparse())),
+    ("dense", lambda: quantize_tokens(torch.zeros(3, 4, dtype=torch.complex64).conj().imag)),
     ("of type", lambda: dequantize_tokens(X, S)),
     ("dtype must be", lambda: dequantize_tokens(Q, S, dtype=torch.int8)),
     ("shape", lambda: dequantize_tokens(Q, S[:3])),
@@ -83,6 +83,9 @@ def _linear_status(**over):
     {"w_stride": 31}, {"y_stride": 7}, {"x_stride": -1}, {"x": None}, {"y": None}, {"w": None}, {"w_scales": None},
     {"x_scales": None}, {"x_type": 0}, {"rows": 2 ** 31}, {"y_type": 3}, {"y_type": 3, "output_scale": float("inf")},
     {"y_type": 3, "output_scale": -1.0},
+    # arrays that do not start on an element
+    {"x_type": 0, "x_scales": None, "x": 4098}, {"x_type": 1, "x_scales": None, "x": 4097}, {"y": 4098},
+    {"y_type": 2, "y": 4097}, {"x_scales": 4097}, {"w_scales": 4098}, {"bias": 4099}, {"y_type": 3, "y_scales": 4098},
     # workspace missing, too small or misaligned
     {"x_type": 0, "x_scales": None}, {"x_type": 0, "x_scales": None, "workspace": 4096, "workspace_bytes": 16},
     {"x_type": 0, "x_scales": None, "workspace": 4097, "workspace_bytes": 1 << 20},
@@ -107,6 +110,8 @@ def test_c_entry_points_do_nothing_for_no_rows():
     (0, None, 0, 4, 8, 8, 4096, 8, 4096, None),
     (0, 4096, 0, 4, 8, 8, 4096, 8, None, None),
     (0, 4096, 0, -1, 8, 8, 4096, 8, 4096, None),
+    (0, 4098, 0, 4, 8, 8, 4096, 8, 4096, None),      # x within an element
+    (0, 4096, 0, 4, 8, 8, 4096, 8, 4097, None),
 ])
 def test_quantise_entry_point_refuses(args):
     assert _lib.load().sc_quantize_tokens_device(*args) == _lib.SC_ERR_INVALID_ARGUMENT
@@ -117,6 +122,8 @@ def test_quantise_entry_point_refuses(args):
     (0, 4096, 8, None, 1.0, 4, 8, 4096, 0, 7, None),
     (0, None, 8, None, 1.0, 4, 8, 4096, 0, 8, None),
     (0, 4096, -8, None, 1.0, 4, 8, 4096, 0, 8, None),
+    (0, 4096, 8, None, 1.0, 4, 8, 4097, 2, 8, None),
+    (0, 4096, 8, 4098, 1.0, 4, 8, 4096, 2, 8, None),
 ])
 def test_dequantise_entry_point_refuses(args):
     assert _lib.load().sc_dequantize_tokens_device(*args) == _lib.SC_ERR_INVALID_ARGUMENT
@@ -124,4 +131,3 @@ def test_dequantise_entry_point_refuses(args):
 
 def test_workspace_size_is_a_whole_number_of_bytes():
     assert isinstance(_lib.load().sc_int8_linear_workspace(1, 1, 1, 1, 512, 8192, 2, 0), int)
-    assert ctypes.sizeof(ctypes.c_int64) == 8
