@@ -11,6 +11,9 @@ counterpart is bit_exact_linear_kernel (sigcomp/quant_mlp_export.py:21-76).  The
 is checked against int32 products requantised like the reference on the smallest M.
 
 Usage (one GPU): ``python -m sigcomp_b200.layer_sweep [--rows 4096,16384,65536,262144,1048576]``
+
+With ``--token-scales`` the same shapes run on ``int8_linear_requant`` (sigcomp_b200.int8): int8 rows
+with a scale for each token and channel in, the same out.
 """
 
 import argparse
@@ -77,13 +80,48 @@ def sweep(rows_list, repeats=5, gpu=0):
     return out
 
 
+def token_scale_sweep(rows_list, repeats=7):
+    """The same shapes with a scale for each token and channel: one call of int8_linear_requant, against
+    ``torch._int_mm``, in CUDA-event time."""
+    import torch
+    from .int8 import int8_linear_requant
+    shapes = (("layer 0 (N=512, K=8192)", 512, 8192), ("hidden (N=512, K=512)", 512, 512), ("last (N=256, K=512)", 256, 512))
+
+    def best(call):
+        call()
+        times = []
+        for _ in range(repeats):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            call()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    out = []
+    for name, n, k in shapes:
+        w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda")
+        scales, bias = torch.rand(n, device="cuda"), torch.rand(n, device="cuda")
+        for m in rows_list:
+            q = torch.randint(-127, 128, (m, k), dtype=torch.int8, device="cuda")
+            s = torch.rand(m, device="cuda")
+            t_layer = best(lambda: int8_linear_requant(q, s, w, scales, bias, relu=True))
+            t_mm = best(lambda: torch._int_mm(q, w.t()))
+            ops = 2.0 * m * n * k
+            out.append((name, m, t_layer, ops / (t_layer * 1e-3) / 1e12, t_mm, ops / (t_mm * 1e-3) / 1e12))
+            del q, s
+    return out
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("--rows", default="4096,16384,65536,262144,1048576")
     ap.add_argument("--repeats", type=int, default=5)
+    ap.add_argument("--token-scales", action="store_true", help="a scale for each token and channel (int8_linear_requant)")
     args = ap.parse_args(argv)
     rows = [int(r) for r in args.rows.split(",")]
-    res = sweep(rows, args.repeats)
+    res = token_scale_sweep(rows) if args.token_scales else sweep(rows, args.repeats)
     print(f"{'shape':28s} {'M':>9s} {'layer ms':>10s} {'layer TOP/s':>12s} {'_int_mm ms':>11s} {'_int_mm TOP/s':>14s}"
           f" {'of 4.5 POPS':>11s}")
     for name, M, tl, al, tm, am in res:

@@ -505,3 +505,9 @@ def test_weights_written_right_before_the_call(ops):
 def test_no_wait_has_timed_out(ops):
     ops.check_waits(DEV)
     ops.check_waits()
+
+
+def test_layer_sweep_with_token_scales():
+    from sigcomp_b200.layer_sweep import token_scale_sweep
+    rows = token_scale_sweep([300], repeats=2)
+    assert [r[0].split(" ")[0] for r in rows] == ["layer", "hidden", "last"] and all(r[2] > 0 and r[4] > 0 for r in rows)
