@@ -167,7 +167,8 @@ __device__ __forceinline__ uint4 first_bytes(uint4 v, int bytes)
 // ---- quantise --------------------------------------------------------------------------------
 // A row is read once: THREADS threads (a part of a warp, a warp or more) hold its 16-byte vectors in registers through
 // the maximum, R rows at a time where rows are short, so that enough loads are in flight.  Bound by HBM
-// (e + 1 bytes per element).
+// (e + 1 bytes per element): 262,144 x 512 fp16 in 61 us, 6.6 TB/s; 20,480 x 8,192 bf16 in 74 us, 6.8 TB/s.  Rows of 511
+// at any address: 112 us, bound by the instructions that shift them.
 template <typename T, int THREADS, int HELD, int R, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
 k_quantize(const T *__restrict__ x, int64_t rows, int cols, int64_t x_stride, int8_t *__restrict__ q, int64_t q_stride,
@@ -312,7 +313,7 @@ k_quantize_long(const T *__restrict__ x, int cols, int64_t x_stride, int8_t *__r
 
 // ---- dequantise ------------------------------------------------------------------------------
 // 16 bytes of results a thread and row, four rows in flight: a block's 256 threads are 2^log_lanes
-// vectors wide.  Bound by HBM (1 + e bytes per element).  Where y's rows do not start on 16 bytes (ALIGNED false), a
+// vectors wide.  Bound by HBM (1 + e bytes per element): 262,144 x 512 to fp16 in 62 us, 6.5 TB/s.  Where y's rows do not start on 16 bytes (ALIGNED false), a
 // row's vectors are those of the addresses, so the first one and the last may be parts, and their bytes
 // of q are read as the three words around them.
 template <typename T, bool ALIGNED>

@@ -30,6 +30,10 @@ using namespace tc;
 // (TOPS), the second quantises by them (BY_TOPS).
 //
 // Every wait is bounded; a warp that gives up ends, and the others end on their own limits.
+//
+// Measured: 65,536 x 8,192 -> 512 bf16 in 171 us (3.2 P operations a second, tensor pipe 89 % active; 214 us in a long
+// loop, where the 1 kW cap holds the clock at 1.18 GHz), 4,096 cubed in 47 to 56 us, 262,144 x 512 -> 512 bf16 in
+// 77 us and requantised in 75 to 87 us, where the epilogue bounds it (ALU 40 %, its passes wait for the products).
 constexpr int PM = 128;                        // rows per CTA
 constexpr int PN = 256;                        // channels per unit
 constexpr int PK = 128;                        // bytes of K per stage
@@ -574,6 +578,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 // the S parts (whole numbers: any order) and writes the results, a warp writing a token's 128 channels at
 // once.  No workspace, no counters, one launch.  (Stores to the owner's memory by each thread, and a cluster
 // barrier, took 10,500 clocks for 64 tokens.)
+//
+// Bound by the latency of its chain (set-up, load, MMA, exchange, store), then by what a few CTAs read of L2: 16 rows of
+// 512 x 512 in 3.4 us, of 8,192 x 512 in 5.1, of 4,096 x 4,096 in 5.9 (2.8 TB/s of weights).
 //
 // Requantised rows (ROWS_OUT): the cluster holds all channels of its tokens, C = n / 128 CTAs with S parts of K
 // each, at most sixteen CTAs; those that own the same tokens exchange their rows' maxima.

@@ -11,7 +11,8 @@ namespace {
 // 512-byte steps, two steps ahead, multiplying with dp4a against the tokens in shared memory; a token's
 // vector is read once for the four channels.  The first steps are requested before the tokens are there.
 // Float tokens are quantised on the way to shared memory by every CTA for itself, which costs a
-// reading of the token from L2 and saves a launch.
+// reading of the token from L2 and saves a launch.  One token: 3.1 us for 512 x 512, 3.7 for 8,192 x 512 (4.9 from bf16),
+// 4.6 for 4,096 x 4,096 (3.6 TB/s); k_few takes 3.3, 5.1 and 5.9.
 struct TokenParams {
     const void *x;
     int64_t x_stride;

@@ -511,3 +511,38 @@ def test_layer_sweep_with_token_scales():
     from sigcomp_b200.layer_sweep import token_scale_sweep
     rows = token_scale_sweep([300], repeats=2)
     assert [r[0].split(" ")[0] for r in rows] == ["layer", "hidden", "last"] and all(r[2] > 0 and r[4] > 0 for r in rows)
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Arrays of more than 2**32 elements: their last rows come out as they do alone."""
+    rows, k = 540000, 8192
+    q = torch.zeros((rows, k), dtype=torch.int8, device=DEV)
+    s = torch.ones(rows, device=DEV)
+    tail, ts = int8_rows(300, k, 1), scales_of(300, 2)
+    q[-300:], s[-300:] = tail, ts
+    w, ws, b = layer(24, k, 3)
+    y = ops.int8_linear(q, w, ws, b, x_scales=s)
+    assert torch.equal(y[-300:], ops.int8_linear(tail, w, ws, b, x_scales=ts)) and torch.equal(y[0], b)
+    x = ops.dequantize_tokens(q, s, dtype=torch.bfloat16)
+    del q
+    assert torch.equal(x[-300:], ops.dequantize_tokens(tail, ts, dtype=torch.bfloat16)) and not x[-301].any()
+    again, scales = ops.quantize_tokens(x)
+    want, wscales = ops.quantize_tokens(x[-300:])
+    assert torch.equal(again[-300:], want) and torch.equal(scales[-300:], wscales) and not again[-301].any()
+
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("rows,n", [(3, 40), (70, 512), (6000, 300), (6000, 512), (6000, 900)])
+def test_requantised_rows_of_extreme_results(ops, relu, rows, n):
+    """Results far below zero, infinite or NaN through the bias, and rows that ReLU leaves empty."""
+    q, s = int8_rows(rows, 64, 1), scales_of(rows, 2)
+    w, ws, _ = layer(n, 64, 3)
+    for value in (-1e30, float("-inf"), float("inf"), float("nan"), -1.0):
+        b = torch.zeros(n, device=DEV) if value != -1.0 else torch.full((n,), -50.0, device=DEV)
+        b[n // 2] = value
+        with np.errstate(invalid="ignore", over="ignore"):
+            y = want_linear(host(q), host(s), host(w), host(ws), host(b), relu)
+        wq, wscale = want_quantized(y)
+        yq, ys = ops.int8_linear_requant(q, s, w, ws, b, relu=relu)
+        same(ys, wscale)
+        same(yq, wq)
