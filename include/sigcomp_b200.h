@@ -336,7 +336,8 @@ SC_API int sc_int8_linear_device(int device, const void *x, int32_t x_type, int6
 
 /* Workspace of a call with these arguments (host only).  x_packed (for an int8 x) and w_packed:
  * nonzero when the address and the stride are multiples of 16 and rows do not overlap; arrays
- * that are not are copied into the workspace first.  y_scaled: nonzero when y_scales is given. */
+ * that are not are copied into the workspace first.  y_scaled: nonzero when y_scales is given.
+ * 0 for arguments that the call refuses. */
 SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_packed, int64_t rows, int64_t n,
                                         int64_t k, int32_t y_type, int32_t y_scaled);
 

@@ -810,6 +810,9 @@ int sc_dequantize_tokens_device(int device, const int8_t *q, int64_t q_stride, c
 int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_packed, int64_t rows, int64_t n, int64_t k,
                                  int32_t y_type, int32_t y_scaled)
 {
+    if (x_type < SC_TYPE_F32 || x_type > SC_TYPE_I8 || y_type < SC_TYPE_F32 || y_type > SC_TYPE_I8 ||
+        k > SC_INT8_MAX_K || !rows_ok(rows, n, n) || !rows_ok(n, k, k) || rows == 0)
+        return 0;
     Int8Linear p{};
     float some = 0;
     p.x_type = x_type;
@@ -820,7 +823,7 @@ int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_pac
     p.k = k;
     p.y_type = y_type;
     p.y_scales = y_scaled ? &some : nullptr;
-    return rows > 0 ? int8_linear_workspace(p) : 0;
+    return int8_linear_workspace(p);
 }
 
 int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_stride, const float *x_scales,

@@ -131,3 +131,24 @@ def test_dequantise_entry_point_refuses(args):
 
 def test_workspace_size_is_a_whole_number_of_bytes():
     assert isinstance(_lib.load().sc_int8_linear_workspace(1, 1, 1, 1, 512, 8192, 2, 0), int)
+
+
+@pytest.mark.parametrize("args", [
+    (3, 1, 1, 4, 0, 32, 0, 0), (3, 1, 1, 4, 8, 0, 0, 0), (3, 1, 1, -4, 8, 32, 0, 0), (3, 1, 1, 4, -1, 32, 3, 1),
+    (9, 1, 1, 4, 8, 32, 0, 0), (3, 1, 1, 4, 8, 32, -1, 0), (0, 1, 1, 4, 8, 1 << 40, 0, 0), (0, 0, 0, 1 << 60, 8, 8, 3, 1),
+])
+def test_workspace_of_refused_arguments(args):
+    assert _lib.load().sc_int8_linear_workspace(*args) == 0
+
+
+def test_workspace_sizes():
+    """Rows of 8 bits and their scales, spread arrays, a product in 32 bits: each where it is needed."""
+    size = _lib.load().sc_int8_linear_workspace
+    assert size(3, 1, 1, 1000, 512, 512, 0, 0) == 0
+    assert size(0, 0, 1, 1000, 512, 500, 0, 0) == 1000 * 512 + 4096                     # rounded to 256 bytes
+    assert size(3, 0, 1, 1000, 512, 500, 0, 0) == 1000 * 512
+    assert size(3, 1, 0, 1000, 512, 500, 0, 0) == 512 * 512
+    assert size(0, 0, 1, 1, 512, 500, 0, 0) == 0                                        # one token: quantised on the way
+    for rows in (1, 16, 300, 5000, 100000):
+        for n in (3, 512, 2000):
+            assert 0 <= size(3, 1, 1, rows, n, 256, 3, 1) <= rows * (n + 3) * 4 + 256
