@@ -444,6 +444,49 @@ __device__ __forceinline__ uint32_t static_bits(float y, float scale)
     return (uint32_t)o & 0xffu;
 }
 
+__device__ __forceinline__ uint32_t static_bits(uint32_t y, float least, float scale)
+{
+    const float v = __uint_as_float(y);
+    return static_bits(least == 0.0f ? max_nan(v, 0.0f) : v, scale);
+}
+
+// The same for 32 results, after ReLU where `least` is 0 and not -128: y times the rounded reciprocal is within 2.3e-5 of
+// y / scale below 128, so only a product that close to a half, or one that is no number, needs the division
+// (about one of 17,000), and then all 32 are divided.  usual: whether the reciprocal is that near.
+__device__ __forceinline__ void static32(const uint32_t (&y)[32], float scale, float inv, bool usual, float least,
+                                         uint32_t (&o)[8])
+{
+    bool exact = usual;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float t = __fmul_rn(__uint_as_float(y[4 * i + j]), inv);
+            float c;
+            asm("max.NaN.f32 %0, %1, %2;\n\tmin.NaN.f32 %0, %0, 0f42FE0000;" : "=&f"(c) : "f"(t), "f"(least));     // 127
+            const float v = __fadd_rn(c, kMagic), d = __fsub_rn(c, __fsub_rn(v, kMagic));
+            exact = exact && fabsf(d) <= 0.49997f;
+            b[j] = __float_as_uint(v);
+        }
+        o[i] = pack4(b[0], b[1], b[2], b[3]);
+    }
+    if (!exact) {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k == i)
+                    w = pack4(static_bits(y[4 * k], least, scale), static_bits(y[4 * k + 1], least, scale),
+                              static_bits(y[4 * k + 2], least, scale), static_bits(y[4 * k + 3], least, scale));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k == i) o[k] = w;
+        }
+    }
+}
+
 }  // namespace
 }  // namespace sc
 
@@ -545,6 +588,7 @@ void quantize(const T *x, int64_t rows, int cols, int64_t xs, int8_t *q, int64_t
     else if (vecs <= 64 && !few) launch_quantize<T, 32, 2, 2>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128 && !few) launch_quantize<T, 32, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 128) launch_quantize<T, 128, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
+    else if (vecs <= 256 && !few) launch_quantize<T, 128, 2, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 512 && !few) launch_quantize<T, 128, 4, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 256 && few) launch_quantize<T, 256, 1, 1>(x, rows, cols, xs, q, qs, scales, s);
     else if (vecs <= 1024 && few) launch_quantize<T, 1024, 1, 1>(x, rows, cols, xs, q, qs, scales, s);

@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 }
                 __syncwarp();
             }
-            if constexpr (MODE == PLAIN || MODE == STATIC) {
+            if constexpr (MODE == PLAIN) {
                 const int ab = uu & 1;
                 const int col0 = block * PN + grp * (PN / 2);
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_cluster(&acc_full[ab], (uu >> 1) & 1)))) break;
@@ -421,10 +421,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                                 const float y1 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2) + 1]);
                                 const uint32_t r = rl + 8 * i, at = (h + 8 * j + 2 * cl) * (uint32_t)sizeof(T);
                                 uint8_t *to = tile + sw128_offset(r, at >> 4) + (at & 15);
-                                if constexpr (MODE == STATIC)
-                                    *reinterpret_cast<uint16_t *>(to) =
-                                        (uint16_t)(static_bits(y0, p.output_scale) | static_bits(y1, p.output_scale) << 8);
-                                else if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(to) = make_float2(y0, y1);
+                                if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(to) = make_float2(y0, y1);
                                 else *reinterpret_cast<uint32_t *>(to) = pack2(y0, y1, T());
                             }
                     }
@@ -455,7 +452,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int i = 0; i < 4 && MODE != BY_TOPS; ++i) {
+                            for (int i = 0; i < 4 && MODE != BY_TOPS && MODE != STATIC; ++i) {
                                 const float y0 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2)]);
                                 const float y1 = __uint_as_float(v[i / 2][4 * j + 2 * (i % 2) + 1]);
                                 top[i] = p.relu ? max3_nan(top[i], y0, y1) : max3_abs_nan(top[i], y0, y1);
@@ -483,7 +480,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 uint32_t largest = 0;
                 if constexpr (MODE == BY_TOPS) {
                     if (row0 + lane < p.rows) largest = p.tops[row0 + lane];
-                } else {
+                } else if constexpr (MODE == ROWS) {
                     // the row's other half of the columns is with the other warp of this quarter, which
                     // cannot be more than one tile ahead: two parities of the buffer are enough
                     float *mx = row_max + (step & 1) * 2 * PM;
@@ -500,17 +497,20 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                 }
                 // from here on a thread has a row of its own: its results lie in 16 bytes at a time
                 const RowScale rs = row_scale(largest);
-                if (grp == 0 && first_block == 0 && row0 + lane < p.rows) p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
+                if (MODE != STATIC && grp == 0 && first_block == 0 && row0 + lane < p.rows) p.y_scales[row0 + lane] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
                 const bool all_finite = __all_sync(0xffffffffu, rs.finite);
-                const float least = p.relu ? kMagic : -INFINITY;
+                const float least = MODE == STATIC ? (p.relu ? 0.0f : -128.0f) : p.relu ? kMagic : -INFINITY;
+                const float inv = __fdiv_rn(1.0f, p.output_scale);                       // STATIC
+                const bool usual = p.output_scale >= 0x1p-100f && p.output_scale <= 0x1p100f;
                 for (int h = 0; h < halves; ++h) {
                     const int ab = (uu + h) & 1;
                     const int live = p.n - (first_block + h) * PN - grp * (PN / 2);
                     staging_free(p, lane);
                     auto scale32 = [&](const uint32_t(&now)[32], int c) {
                         uint32_t o[8];
+                        if constexpr (MODE == STATIC) static32(now, p.output_scale, inv, usual, least, o);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
+                        for (int i = 0; i < 8 && MODE != STATIC; ++i) {
                             F2 z[2];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                             o[i] = pack4(__float_as_uint(z[0].x), __float_as_uint(z[0].y), __float_as_uint(z[1].x),
                                          __float_as_uint(z[1].y));
                         }
-                        if (!all_finite && !rs.finite) {
+                        if (MODE != STATIC && !all_finite && !rs.finite) {
 #pragma unroll
                             for (int i = 0; i < 8; ++i) o[i] = 0;
                         }

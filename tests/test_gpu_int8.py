@@ -546,3 +546,25 @@ def test_requantised_rows_of_extreme_results(ops, relu, rows, n):
         yq, ys = ops.int8_linear_requant(q, s, w, ws, b, relu=relu)
         same(ys, wscale)
         same(yq, wq)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 6000])
+@pytest.mark.parametrize("scale", [0.06, 1.0, 0.011, 3.7, 2.0 ** -120, 3e30, 1.1e-38])
+@pytest.mark.parametrize("relu", [False, True])
+def test_logits_next_to_a_half(ops, rows, scale, relu):
+    """Results at halves of the output scale, next to them on both sides, beyond the ends, and no numbers."""
+    scale32 = np.float32(scale)
+    half = (np.arange(-131, 131, dtype=np.float64) + 0.5) * np.float64(scale32)
+    with np.errstate(over="ignore"):
+        at = half.astype(np.float32)
+        values = np.concatenate([np.nextafter(at, np.float32(-np.inf)), at, np.nextafter(at, np.float32(np.inf)),
+                                 np.float32([np.nan, np.inf, -np.inf, 0, -0.0, 1e38, -1e38, 1e-40, -1e-45])])
+    n = len(values)
+    q, s = torch.zeros((rows, 64), dtype=torch.int8, device=DEV), torch.ones(rows, device=DEV)
+    w, ws, _ = layer(n, 64, 3)
+    got = ops.int8_linear_requant(q, s, w, ws, torch.from_numpy(values).to(DEV), relu=relu, output_scale=float(scale32))
+    y = np.where(values < 0, np.float32(0), values) if relu else values
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = np.clip(np.rint(y / scale32), -128, 127)
+    want = np.where(np.isnan(want), 0, want).astype(np.int8)
+    same(got, np.tile(want, (rows, 1)))
