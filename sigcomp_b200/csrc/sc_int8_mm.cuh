@@ -27,7 +27,8 @@ using namespace tc;
 // tile's half 0.
 //
 // Rows of more channels are quantised by two launches that both multiply: the first keeps the rows' largest magnitudes
-// (TOPS), the second quantises by them (BY_TOPS).
+// (TOPS), the second quantises by them (BY_TOPS).  Those and rows quantised by one scale (STATIC) go unit by unit through
+// the same two passes, without a maximum, so that a row's bytes are staged sixteen at a time.
 //
 // Every wait is bounded; a warp that gives up ends, and the others end on their own limits.
 //
