@@ -446,6 +446,13 @@ __global__ void __launch_bounds__(P_THREADS, 1) k_pair(const __grid_constant__ P
                         tmem_ld_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
                         tmem_ld_wait();
                         affine_16x32(v, reinterpret_cast<const float4 *>(tb + h * PN) + c / 2 + cl, s);
+                        // columns behind the last channel are no results: sums of zero, which an infinite scale of the
+                        // row makes NaN, stay out of its maximum
+                        if ((MODE == ROWS || MODE == TOPS) && c + 32 > live) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (c + i / 8 * 8 + 2 * cl + i % 2 >= live) v[i / 4 % 2][i / 8 * 4 + i / 2 % 2 * 2 + i % 2] = 0;
+                        }
                         if (MODE != TOPS) {
                             tmem_st_16x32(lane_base + ab * PN + c, v[0]);
                             tmem_st_16x32(lane_base + (16u << 16) + ab * PN + c, v[1]);
@@ -843,9 +850,11 @@ __global__ void __launch_bounds__(FewCfg<BT>::THREADS, 1) k_few(const __grid_con
                     const int j = warp - 2 + C::EPI * u;
                     if (j >= own) break;
                     results(j, y[u]);
-                    uint32_t top = 0;                                  // channels behind the last one are 0, or NaN with the row
+                    // channels behind the last one are sums of zero, which an infinite scale of the row makes NaN
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) top = max(top, magnitude(y[u][i]));
+                    for (int i = 0; i < 4; ++i)
+                        if (ch + i < p.n) top = max(top, magnitude(y[u][i]));
                     top = __reduce_max_sync(0xffffffffu, top);
                     if (lane < tiles) {
                         const uint32_t at = map_to_rank(mx + tile0 / S * BT + j, (uint32_t)(lane * S + part));

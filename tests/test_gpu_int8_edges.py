@@ -1,0 +1,42 @@
+"""The int8 operators on a GPU at calls that their first tests leave out, against the same definition."""
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_int8 import DEV, host, layer, same, want_linear, want_quantized
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from sigcomp_b200 import int8
+    return int8
+
+
+# ---- infinite scales ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("k,n", [(64, 1), (64, 33), (64, 40), (512, 130), (512, 300), (96, 500), (96, 900), (64, 512)])
+def test_infinite_scales_of_rows(ops, k, n, relu):
+    """Rows whose scale is infinite: sums below zero are minus infinity, which ReLU makes 0, so the row can be
+    quantised; sums above zero and sums of zero (a NaN) make it one that cannot be.  The same in a batch of any size."""
+    kinds = 6
+    q = torch.zeros((kinds, k), dtype=torch.int8, device=DEV)
+    q[0], q[1], q[2, 0], q[4], q[5] = 1, -1, 0, 1, 100          # row 2: sums of zero; 3: an ordinary row of zeros
+    s = torch.tensor([np.inf, np.inf, np.inf, 1.0, -np.inf, 0.5], device=DEV)
+    w = torch.full((n, -(-k // 16) * 16), -1, dtype=torch.int8, device=DEV)[:, :k]
+    w[n // 2] = -3
+    _, ws, b = layer(n, k, 3)
+    with np.errstate(invalid="ignore", over="ignore"):
+        y = want_linear(host(q), host(s), host(w), host(ws), host(b), relu)
+    wq, wscale = want_quantized(y)
+    assert np.isfinite(wscale[0]) == relu and np.isnan(wscale[1:3]).all()
+    for rows in (1, 2, 3, 6, 40, 700, 6000, 20000):
+        pick = torch.arange(rows, device=DEV) % kinds
+        idx = pick.cpu().numpy()
+        yq, ys = ops.int8_linear_requant(q[pick], s[pick], w, ws, b, relu=relu)
+        same(ys, wscale[idx])
+        same(yq, wq[idx])
+        same(ops.int8_linear(q[pick], w, ws, b, x_scales=s[pick], relu=relu), y[idx])
