@@ -8,6 +8,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -67,6 +68,9 @@ const at::Tensor &tensor(const char *name, PyObject *o, int types, const at::Ten
         refuse("%s is on %s, the other arrays are on %s", name, t.device().str().c_str(), beside->device().str().c_str());
     if (t.requires_grad() && c10::GradMode::is_enabled())
         refuse("%s asks for a gradient, which the int8 operators do not have", name);
+    // a dual tensor: its tangent would be lost
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        refuse("%s asks for a forward derivative, which the int8 operators do not have", name);
     return t;
 }
 

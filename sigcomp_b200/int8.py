@@ -19,7 +19,8 @@ Arrays are torch tensors on one GPU; leading dimensions are batch dimensions.  R
 start a multiple of 16 bytes apart, so results are contiguous where their width is such a multiple, and
 strided otherwise (rows of odd widths side by side took two to five times as long to write).  Work is put into the
 current stream of that GPU and not waited for, so calls can be captured into CUDA graphs.  The
-operators serve coding, not training: a tensor that asks for a gradient is refused.
+operators serve coding, not training: a tensor that asks for a gradient, or carries a tangent
+(``torch.autograd.forward_ad``), is refused.
 """
 
 import torch

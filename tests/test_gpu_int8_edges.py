@@ -40,3 +40,21 @@ def test_infinite_scales_of_rows(ops, k, n, relu):
         same(ys, wscale[idx])
         same(yq, wq[idx])
         same(ops.int8_linear(q[pick], w, ws, b, x_scales=s[pick], relu=relu), y[idx])
+
+
+# ---- derivatives and batching by torch ---------------------------------------------------------
+
+def test_tangents_and_transforms_are_refused(ops):
+    """A dual tensor's tangent would be lost, and a batched one has no memory of its own."""
+    x, (w, ws, b) = torch.randn(4, 64, device=DEV), layer(32, 64, 1)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match="derivative"):
+            ops.int8_linear(dual, w, ws, b)
+        assert torch.equal(ops.int8_linear(torch.autograd.forward_ad.unpack_dual(dual).primal, w, ws, b),
+                           ops.int8_linear(x, w, ws, b))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: ops.int8_linear(v, w, ws, b))(x)
+    for transform in (torch.func.grad, torch.func.jacfwd):
+        with pytest.raises(ValueError, match="gradient|derivative"):
+            transform(lambda v: ops.int8_linear(v, w, ws, b).sum())(x)

@@ -1,0 +1,51 @@
+"""Refusals of the int8 operators that need no GPU, beyond the plain ones."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from sigcomp_b200.int8 import dequantize_tokens, int8_linear, int8_linear_requant, quantize_tokens
+
+X = torch.zeros((4, 32))
+Q = torch.zeros((4, 32), dtype=torch.int8)
+S = torch.ones(4)
+W = torch.zeros((8, 32), dtype=torch.int8)
+T = torch.ones(8)
+B = torch.zeros(8)
+
+
+# ---- forward-mode derivatives ------------------------------------------------------------------
+
+CALLS = {
+    "quantize": (X, lambda d: quantize_tokens(d)),
+    "dequantize scales": (S, lambda d: dequantize_tokens(Q, d)),
+    "linear x": (X, lambda d: int8_linear(d, W, T, B)),
+    "linear weight_scales": (T, lambda d: int8_linear(X, W, d, B)),
+    "linear bias": (B, lambda d: int8_linear(X, W, T, d)),
+    "linear x_scales": (S, lambda d: int8_linear(Q, W, T, B, x_scales=d)),
+    "requant scales": (S, lambda d: int8_linear_requant(Q, d, W, T)),
+    "requant bias": (B, lambda d: int8_linear_requant(Q, S, W, T, d)),
+}
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tangents_are_refused(name):
+    """A dual tensor asks for a derivative in the forward direction, also where no gradient is recorded."""
+    primal, call = CALLS[name]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(primal, torch.ones_like(primal))
+        with pytest.raises(ValueError, match="derivative"):
+            call(dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="derivative"):
+            call(dual)
+        with pytest.raises(ValueError, match="run on a GPU"):
+            call(forward_ad.unpack_dual(dual).primal)
+
+
+@pytest.mark.parametrize("transform", [
+    lambda f: torch.func.jvp(f, (X,), (torch.ones_like(X),)), lambda f: torch.func.grad(f)(X),
+    lambda f: torch.func.jacfwd(f)(X), lambda f: torch.func.jacrev(f)(X),
+])
+def test_derivatives_by_function_transforms_are_refused(transform):
+    with pytest.raises((ValueError, RuntimeError), match="derivative|gradient|storage"):
+        transform(lambda x: int8_linear(x, W, T).sum())
