@@ -81,10 +81,14 @@ std::string shape_of(c10::IntArrayRef s)
     return o + (s.size() == 1 ? ",)" : ")");
 }
 
-// t as rows: a view where its strides allow one, else a copy
-at::Tensor as_rows(const char *name, const at::Tensor &t)
+void rows_there(const char *name, const at::Tensor &t)
 {
     if (t.dim() == 0 || t.size(-1) == 0) refuse("%s must have rows of at least one element", name);
+}
+
+// t as rows: a view where its strides allow one, else a copy
+at::Tensor as_rows(const at::Tensor &t)
+{
     at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
     return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
@@ -99,7 +103,7 @@ at::Tensor vector_of(const char *name, PyObject *o, int64_t length, const at::Te
     const at::Tensor &t = tensor(name, o, F32, &beside);
     if (t.dim() != 1 || t.size(0) != length)
         refuse("%s must have %lld elements, not shape %s", name, (long long)length, shape_of(t.sizes()).c_str());
-    return t.is_contiguous() ? t : t.contiguous();
+    return t;
 }
 
 at::Tensor row_scales(const char *name, PyObject *o, c10::IntArrayRef lead, const at::Tensor &beside)
@@ -107,7 +111,14 @@ at::Tensor row_scales(const char *name, PyObject *o, c10::IntArrayRef lead, cons
     const at::Tensor &t = tensor(name, o, F32, &beside);
     if (t.sizes() != lead)
         refuse("%s must have shape %s, one scale for each row, not %s", name, shape_of(lead).c_str(), shape_of(t.sizes()).c_str());
-    return t.is_contiguous() ? t : t.contiguous();
+    return t;
+}
+
+const float *floats_of(at::Tensor &t)
+{
+    if (!t.defined()) return nullptr;
+    if (!t.is_contiguous()) t = t.contiguous();
+    return (const float *)t.data_ptr();
 }
 
 at::Tensor empty(c10::IntArrayRef sizes, c10::ScalarType type, const at::Tensor &beside)
@@ -142,6 +153,13 @@ c10::IntArrayRef leading(const at::Tensor &t) { return t.sizes().slice(0, t.dim(
 // the distance of rows; of a single row any distance will do, and its own length is always a valid one
 int64_t row_stride(const at::Tensor &rows) { return rows.size(0) > 1 ? rows.stride(0) : (rows.size(1) + 15) / 16 * 16; }
 
+// Other Python threads run meanwhile, as they do during torch's own calls: an allocation can wait for the GPU, and so
+// can a launch where the stream's queue is full, perhaps for work that another thread has yet to launch.
+struct Unlocked {
+    PyThreadState *state = PyEval_SaveThread();
+    ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 struct Failed {
     int status;
 };
@@ -174,21 +192,28 @@ PyObject *pair(at::Tensor a, at::Tensor b)
 
 PyObject *quantize(PyObject *const *a)
 {
-    const at::Tensor &x = tensor("x", a[0], FLOATS);
-    at::Tensor rows = as_rows("x", x);
+    const at::Tensor x = tensor("x", a[0], FLOATS);
+    rows_there("x", x);
     on_gpu(x);
-    at::Tensor q = empty_rows(leading(x), x.size(-1), c10::ScalarType::Char, x), s = empty(leading(x), c10::ScalarType::Float, x);
-    check(sc_quantize_tokens_device(x.device().index(), rows.data_ptr(), sc_type(x.scalar_type()), rows.size(0), rows.size(1),
-                                    row_stride(rows), (int8_t *)q.data_ptr(), padded(x.size(-1), c10::ScalarType::Char),
-                                    (float *)s.data_ptr(), stream_of(x)));
+    at::Tensor q, s;
+    {
+        Unlocked unlocked;
+        at::Tensor rows = as_rows(x);
+        q = empty_rows(leading(x), x.size(-1), c10::ScalarType::Char, x);
+        s = empty(leading(x), c10::ScalarType::Float, x);
+        check(sc_quantize_tokens_device(x.device().index(), rows.data_ptr(), sc_type(x.scalar_type()), rows.size(0), rows.size(1),
+                                        row_stride(rows), (int8_t *)q.data_ptr(), padded(x.size(-1), c10::ScalarType::Char),
+                                        (float *)s.data_ptr(), stream_of(x)));
+    }
     return pair(std::move(q), std::move(s));
 }
 
 PyObject *dequantize(PyObject *const *a)
 {
-    const at::Tensor &q = tensor("q", a[0], I8);
+    const at::Tensor q = tensor("q", a[0], I8);
     const c10::ScalarType type = float_type(a[2], c10::ScalarType::Float, "");
-    at::Tensor rows = as_rows("q", q), scales;
+    rows_there("q", q);
+    at::Tensor scales, y;
     double one = 0;
     if (THPVariable_Check(a[1])) {
         scales = row_scales("scales", a[1], leading(q), q);
@@ -197,17 +222,21 @@ PyObject *dequantize(PyObject *const *a)
         if (one == -1.0 && PyErr_Occurred()) return nullptr;
     }
     on_gpu(q);
-    at::Tensor y = empty_rows(leading(q), q.size(-1), type, q);
-    check(sc_dequantize_tokens_device(q.device().index(), (const int8_t *)rows.data_ptr(), row_stride(rows),
-                                      scales.defined() ? (const float *)scales.data_ptr() : nullptr, (float)one, rows.size(0),
-                                      rows.size(1), y.data_ptr(), sc_type(type), padded(q.size(-1), type), stream_of(q)));
+    {
+        Unlocked unlocked;
+        at::Tensor rows = as_rows(q);
+        y = empty_rows(leading(q), q.size(-1), type, q);
+        check(sc_dequantize_tokens_device(q.device().index(), (const int8_t *)rows.data_ptr(), row_stride(rows),
+                                          floats_of(scales), (float)one, rows.size(0), rows.size(1), y.data_ptr(),
+                                          sc_type(type), padded(q.size(-1), type), stream_of(q)));
+    }
     return THPVariable_Wrap(std::move(y));
 }
 
 // x, x_scales, weight, weight_scales, bias, relu, then as y_type says: the type's object, or output_scale
 PyObject *linear(PyObject *const *a, bool int8_out)
 {
-    const at::Tensor &x = tensor(int8_out ? "q" : "x", a[0], int8_out ? I8 : FLOATS | I8);
+    const at::Tensor x = tensor(int8_out ? "q" : "x", a[0], int8_out ? I8 : FLOATS | I8);
     const bool quantised = x.scalar_type() == c10::ScalarType::Char;
     c10::ScalarType type = c10::ScalarType::Char;
     double output_scale = 0;
@@ -220,13 +249,13 @@ PyObject *linear(PyObject *const *a, bool int8_out)
             refuse("output_scale must be a finite positive number");
     }
     const bool row_out = int8_out && a[6] == Py_None;
-    const at::Tensor &weight = tensor("weight", a[2], I8, &x);
+    const at::Tensor weight = tensor("weight", a[2], I8, &x);
     if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0) refuse("weight must be [out, in], both at least 1");
     const int64_t n = weight.size(0), k = weight.size(1);
     if (k > SC_INT8_MAX_K) refuse("rows of more than %d elements could overflow a 32-bit sum", SC_INT8_MAX_K);
     if (x.dim() == 0 || x.size(-1) != k)
         refuse("x has shape %s, weight takes rows of %lld", shape_of(x.sizes()).c_str(), (long long)k);
-    at::Tensor ws = vector_of("weight_scales", a[3], n, x), bias, xs;
+    at::Tensor ws = vector_of("weight_scales", a[3], n, x), bias, xs, y, y_scales;
     if (a[4] != Py_None) bias = vector_of("bias", a[4], n, x);
     if (quantised) {
         if (a[1] == Py_None) refuse("int8 rows need x_scales");
@@ -237,24 +266,25 @@ PyObject *linear(PyObject *const *a, bool int8_out)
     const int relu = PyObject_IsTrue(a[5]);
     if (relu < 0) return nullptr;
     on_gpu(x);
-    at::Tensor rows = as_rows("x", x), w = as_rows("weight", weight);
-    if (n > 1 && w.stride(0) < k) w = w.contiguous();       // rows that overlap, as those of an expanded row do
-    const int64_t m = rows.size(0), x_stride = row_stride(rows), w_stride = row_stride(w);
-    const int xt = sc_type(x.scalar_type()), yt = sc_type(type);
-    at::Tensor y = empty_rows(leading(x), n, type, x), y_scales, work;
-    const int64_t y_stride = padded(n, type);
-    if (row_out) y_scales = empty(leading(x), c10::ScalarType::Float, x);
-    const int x_packed = ((uintptr_t)rows.data_ptr() | (uintptr_t)x_stride) % 16 == 0 && x_stride >= k;
-    const int w_packed = ((uintptr_t)w.data_ptr() | (uintptr_t)w_stride) % 16 == 0;
-    const int64_t bytes = sc_int8_linear_workspace(xt, x_packed, w_packed, m, n, k, yt, row_out);
-    if (bytes > 0) work = empty({bytes}, c10::ScalarType::Byte, x);
-    if (m > 0)
-        check(sc_int8_linear_device(x.device().index(), rows.data_ptr(), xt, x_stride,
-                                    quantised ? (const float *)xs.data_ptr() : nullptr, (const int8_t *)w.data_ptr(), w_stride,
-                                    (const float *)ws.data_ptr(), bias.defined() ? (const float *)bias.data_ptr() : nullptr,
-                                    m, n, k, relu, y.data_ptr(), yt, y_stride,
-                                    row_out ? (float *)y_scales.data_ptr() : nullptr, (float)output_scale,
-                                    bytes > 0 ? work.data_ptr() : nullptr, bytes, stream_of(x)));
+    {
+        Unlocked unlocked;
+        at::Tensor rows = as_rows(x), w = as_rows(weight), work;
+        if (n > 1 && w.stride(0) < k) w = w.contiguous();       // rows that overlap, as those of an expanded row do
+        const int64_t m = rows.size(0), x_stride = row_stride(rows), w_stride = row_stride(w);
+        const int xt = sc_type(x.scalar_type()), yt = sc_type(type);
+        y = empty_rows(leading(x), n, type, x);
+        const int64_t y_stride = padded(n, type);
+        if (row_out) y_scales = empty(leading(x), c10::ScalarType::Float, x);
+        const int x_packed = ((uintptr_t)rows.data_ptr() | (uintptr_t)x_stride) % 16 == 0 && x_stride >= k;
+        const int w_packed = ((uintptr_t)w.data_ptr() | (uintptr_t)w_stride) % 16 == 0;
+        const int64_t bytes = sc_int8_linear_workspace(xt, x_packed, w_packed, m, n, k, yt, row_out);
+        if (bytes > 0) work = empty({bytes}, c10::ScalarType::Byte, x);
+        if (m > 0)
+            check(sc_int8_linear_device(x.device().index(), rows.data_ptr(), xt, x_stride, floats_of(xs),
+                                        (const int8_t *)w.data_ptr(), w_stride, floats_of(ws), floats_of(bias), m, n, k, relu,
+                                        y.data_ptr(), yt, y_stride, row_out ? (float *)y_scales.data_ptr() : nullptr,
+                                        (float)output_scale, bytes > 0 ? work.data_ptr() : nullptr, bytes, stream_of(x)));
+    }
     if (row_out) return pair(std::move(y), std::move(y_scales));
     return THPVariable_Wrap(std::move(y));
 }

@@ -1,5 +1,8 @@
 """The int8 operators on a GPU at calls that their first tests leave out, against the same definition."""
 
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
@@ -58,3 +61,35 @@ def test_tangents_and_transforms_are_refused(ops):
     for transform in (torch.func.grad, torch.func.jacfwd):
         with pytest.raises(ValueError, match="gradient|derivative"):
             transform(lambda v: ops.int8_linear(v, w, ws, b).sum())(x)
+
+
+# ---- host side ---------------------------------------------------------------------------------
+
+def test_other_threads_run_while_a_call_waits_for_the_stream(ops):
+    """More launches than the driver queues, behind work of about a second: the call that has to wait for room lets
+    the process's other Python threads run."""
+    x, (w, ws, b) = torch.randn(4, 64, device=DEV), layer(32, 64, 1)
+    ops.int8_linear(x, w, ws, b)
+    torch.cuda.synchronize()
+    beats, stop = [], threading.Event()
+
+    def beat():
+        while not stop.is_set():
+            beats.append(time.perf_counter())
+            time.sleep(0.005)
+
+    thread = threading.Thread(target=beat)
+    thread.start()
+    try:
+        torch.cuda._sleep(2_000_000_000)
+        longest = 0.0
+        for _ in range(3000):
+            t = time.perf_counter()
+            ops.int8_linear(x, w, ws, b)
+            longest = max(longest, time.perf_counter() - t)
+        torch.cuda.synchronize()
+    finally:
+        stop.set()
+        thread.join()
+    assert longest > 0.3, "no call had to wait: the test shows nothing"
+    assert np.diff(beats).max() < 0.25
