@@ -343,7 +343,8 @@ SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_
 
 /* Waits for `stream` and reports whether a device-side wait of an int8 operator has timed out on
  * the device since the last such report (SC_ERR_CUDA, as the other entry points report it; the
- * results of the calls since then are not to be used). */
+ * results of the calls since then are not to be used).  A stream that is being captured is refused
+ * (SC_ERR_INVALID_ARGUMENT). */
 SC_API int sc_int8_status_device(int device, void *stream);
 
 /*

@@ -865,6 +865,13 @@ int sc_int8_status_device(int device, void *stream)
 {
     g_err[0] = 0;
     return guarded_on(device, [&]() -> int {
+        // waiting for a stream that is being captured would end the capture
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        SC_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &capture));
+        if (capture != cudaStreamCaptureStatusNone) {
+            set_error("the stream is being captured and cannot be waited for");
+            return SC_ERR_INVALID_ARGUMENT;
+        }
         SC_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
         if (int8_device_error()) {
             set_error("a device-side wait timed out (kernel gave up after its time limit)");

@@ -93,3 +93,49 @@ def test_other_threads_run_while_a_call_waits_for_the_stream(ops):
         thread.join()
     assert longest > 0.3, "no call had to wait: the test shows nothing"
     assert np.diff(beats).max() < 0.25
+
+
+def test_check_of_waits_is_refused_during_a_capture(ops):
+    """It has to wait for the stream, which a capture cannot; the refusal leaves the capture as it is."""
+    x, (w, ws, b) = torch.randn(20, 64, device=DEV), layer(32, 64, 1)
+    want = ops.int8_linear(x, w, ws, b)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.int8_linear(x, w, ws, b)
+        with pytest.raises(ValueError, match="captured"):
+            ops.check_waits()
+    got.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    ops.check_waits()
+
+
+def test_capture_over_two_streams(ops):
+    """Operators on a stream that a capture forks to, and one that reads the results of both after the join."""
+    x = torch.randn(300, 512, device=DEV)
+    a, b, last = layer(512, 512, 1), layer(512, 512, 2), layer(96, 512, 3)
+
+    def run(side):
+        main = torch.cuda.current_stream()
+        q, s = ops.quantize_tokens(x)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            right = ops.int8_linear_requant(q, s, *b, relu=True)
+        left = ops.int8_linear_requant(q, s, *a, relu=True)
+        main.wait_stream(side)
+        return ops.int8_linear(left[0], *last, x_scales=left[1]), ops.int8_linear(right[0], *last, x_scales=right[1])
+
+    side = torch.cuda.Stream()
+    want = [t.clone() for t in run(side)]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = run(side)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, v) for t, v in zip(got, want))
