@@ -342,10 +342,16 @@ SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_
                                         int64_t k, int32_t y_type, int32_t y_scaled);
 
 /* Waits for `stream` and reports whether a device-side wait of an int8 operator has timed out on
- * the device since the last such report (SC_ERR_CUDA, as the other entry points report it; the
- * results of the calls since then are not to be used).  A stream that is being captured is refused
- * (SC_ERR_INVALID_ARGUMENT). */
+ * the device since the calling host thread's last such report, or, in its first, since the library
+ * was loaded (SC_ERR_CUDA, as the other entry points report it; the results of the calls since then
+ * are not to be used).  So each thread that asks learns of it, whichever asks first.  A stream that
+ * is being captured is refused (SC_ERR_INVALID_ARGUMENT). */
 SC_API int sc_int8_status_device(int device, void *stream);
+
+/* Failure-detection self test of the int8 operators, as sc_selftest_wait_timeout: puts one small
+ * kernel into `stream` whose wait nothing will satisfy.  It ends after about 2 s, and
+ * sc_int8_status_device then reports the timeout. */
+SC_API int sc_selftest_int8_wait_timeout(int device, void *stream);
 
 /*
  * Per-launch CUDA-event timing (no counterpart in the reference; instrumentation

@@ -26,7 +26,7 @@ EXPORTS = (
     "sc_reassemble_signal_device", "sc_selftest_wait_timeout", "sc_encode_logits_device",
     "sc_decode_logits_device", "sc_frame_reads", "sc_unframe_reads", "sc_linear_layer_device",
     "sc_quantize_tokens_device", "sc_dequantize_tokens_device", "sc_int8_linear_device",
-    "sc_int8_linear_workspace", "sc_int8_status_device",
+    "sc_int8_linear_workspace", "sc_int8_status_device", "sc_selftest_int8_wait_timeout",
 )
 
 KERNEL_KINDS = ("windows", "layer0", "hidden", "last_layer", "cdf_select", "encode", "compact", "decode_step",
@@ -72,6 +72,7 @@ def load():
                                         i64, vp, f32, vp, i64, vp]
     L.sc_int8_linear_workspace.argtypes = [i32, i32, i32, i64, i64, i64, i32, i32]
     L.sc_int8_status_device.argtypes = [ctypes.c_int, vp]
+    L.sc_selftest_int8_wait_timeout.argtypes = [ctypes.c_int, vp]
     L.sc_int8_linear_workspace.restype = i64
     L.sc_profile_enable.argtypes = [vp, i32]
     L.sc_profile_read.argtypes = [vp, i32, vp, vp, vp]
@@ -88,7 +89,7 @@ def load():
                  "sc_selftest_wait_timeout", "sc_encode_logits_device", "sc_decode_logits_device",
                  "sc_frame_reads", "sc_unframe_reads", "sc_linear_layer_device",
                  "sc_quantize_tokens_device", "sc_dequantize_tokens_device", "sc_int8_linear_device",
-                 "sc_int8_status_device"):
+                 "sc_int8_status_device", "sc_selftest_int8_wait_timeout"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
     return L

@@ -4,6 +4,7 @@
 #include <cfloat>
 #include <cstdarg>
 #include <cstring>
+#include <map>
 #include <memory>
 #include <new>
 
@@ -872,11 +873,24 @@ int sc_int8_status_device(int device, void *stream)
             set_error("the stream is being captured and cannot be waited for");
             return SC_ERR_INVALID_ARGUMENT;
         }
-        SC_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-        if (int8_device_error()) {
+        // the count only grows, so that no thread's report takes another's
+        static thread_local std::map<int, int> reported;
+        const int given_up = int8_waits_given_up((cudaStream_t)stream);
+        int &before = reported[device];
+        if (given_up != before) {
+            before = given_up;
             set_error("a device-side wait timed out (kernel gave up after its time limit)");
             return SC_ERR_CUDA;
         }
+        return SC_OK;
+    });
+}
+
+int sc_selftest_int8_wait_timeout(int device, void *stream)
+{
+    g_err[0] = 0;
+    return guarded_on(device, [&]() -> int {
+        int8_wait_selftest((cudaStream_t)stream);
         return SC_OK;
     });
 }

@@ -969,11 +969,31 @@ void int8_linear(const Int8Linear &p, cudaStream_t s)
     if (o.ways.cut < p.rows) rows_of(o.ways.cut, p.rows - o.ways.cut, o.ways.way[1]);
 }
 
-int int8_device_error()
+namespace {
+
+// A wait that nothing ends: gives up after its time limit, is counted, and the kernel ends.
+__global__ void __launch_bounds__(32) k_int8_wait_selftest()
 {
-    int v = 0, z = 0;
-    SC_CUDA(cudaMemcpyFromSymbol(&v, tc::g_device_error, sizeof(int)));
-    if (v) SC_CUDA(cudaMemcpyToSymbol(tc::g_device_error, &z, sizeof(int)));
+    __shared__ __align__(8) uint64_t bar;
+    next_may_start();
+    previous_done();
+    if (threadIdx.x == 0) {
+        tc::mbar_init(&bar, 1);
+        tc::fence_mbar_init();
+    }
+    __syncwarp();
+    if (threadIdx.x == 0) tc::mbar_wait(&bar, 0);
+}
+
+}  // namespace
+
+void int8_wait_selftest(cudaStream_t s) { launch(k_int8_wait_selftest, 1, 32, 0, s, 1); }
+
+int int8_waits_given_up(cudaStream_t s)
+{
+    int v = 0;
+    SC_CUDA(cudaMemcpyFromSymbolAsync(&v, tc::g_device_error, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    SC_CUDA(cudaStreamSynchronize(s));
     return v;
 }
 

@@ -189,10 +189,13 @@ void fused_decode(sc_model *m, const int64_t *order, int64_t n_rows, const int64
                   const int64_t *lengths, DecState *state, const uint32_t *words, uint8_t *tokens_out,
                   const int64_t *out_off, uint8_t *errors, cudaStream_t s);
 
-// Clears and returns the error flag that a timed-out wait of the int8 operators set on the current device.
-int int8_device_error();
+// Waits for the stream, then the number of waits of the int8 operators that have timed out on the current device since
+// the library was loaded.
+int int8_waits_given_up(cudaStream_t s);
+// One kernel of them whose wait times out.
+void int8_wait_selftest(cudaStream_t s);
 
-// Value of the device error flag set by timed-out waits (optionally cleared).
+// Number of the other kernels' waits that timed out (optionally cleared).
 int read_device_error(int clear);
 
 }  // namespace sc

@@ -10,10 +10,10 @@
 namespace sc {
 namespace tc {
 
-// ---- device error flag (bounded waits that give up set it) -----------------
-// Set through atomicExch by a kernel whose wait timed out; read by the host
-// after every call.  Codes: 1 = mbarrier wait timeout.  Every kernel that
-// uses these waits lives in the translation unit that reads the flag.
+// ---- waits that gave up -----------------------------------------------------
+// Each wait that times out adds one.  Every kernel that uses these waits lives in
+// the translation unit that reads its counter: sc_mlp_tc.cu after every call, which
+// clears it; sc_int8.cu when asked, which only compares it with an earlier value.
 static __device__ int g_device_error = 0;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -63,7 +63,7 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
 }
 
 // Wait for the phase with the given parity to complete.  Gives up after two
-// seconds, sets the device error flag and returns false, so that no wait of
+// seconds, counts itself in g_device_error and returns false, so that no wait of
 // these kernels can hang the GPU.
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
@@ -73,7 +73,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
     while (true) {
         if (mbar_try_wait(bar, parity)) return true;
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            atomicExch(&g_device_error, 1);
+            atomicAdd(&g_device_error, 1);
             return false;
         }
     }
@@ -99,7 +99,7 @@ __device__ __forceinline__ bool counter_wait(const uint32_t *c, uint32_t target)
     while (true) {
         if ((int32_t)(counter_load_acquire(c) - target) >= 0) return true;
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            atomicExch(&g_device_error, 2);
+            atomicAdd(&g_device_error, 1);
             return false;
         }
         __nanosleep(64);
@@ -151,7 +151,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
     while (true) {
         if (mbar_try_wait_cluster(bar, parity)) return true;
         if (globaltimer_ns() - t0 > kWaitLimitNs) {
-            atomicExch(&g_device_error, 1);
+            atomicAdd(&g_device_error, 1);
             return false;
         }
     }

@@ -79,8 +79,8 @@ def int8_linear_requant(q, scales, weight, weight_scales, bias=None, *, relu=Fal
 
 def check_waits(device=None):
     """Wait for the current stream of ``device`` and raise if a kernel of these operators gave up a wait
-    there (2 s, see ``sc_int8_status_device``) since the last such check.  Refused while that stream is
-    captured."""
+    there (2 s, see ``sc_int8_status_device``) since this thread's last such check, or, in its first, at any
+    time before.  Refused while that stream is captured."""
     device = torch.device("cuda" if device is None else device)
     index = torch.cuda.current_device() if device.index is None else device.index
     _lib.check(_lib.load().sc_int8_status_device(index, torch.cuda.current_stream(index).cuda_stream),

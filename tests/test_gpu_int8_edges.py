@@ -139,3 +139,42 @@ def test_capture_over_two_streams(ops):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(t, v) for t, v in zip(got, want))
+
+
+# ---- waits that give up ------------------------------------------------------------------------
+
+def test_a_wait_that_gives_up_is_reported_to_every_thread(ops):
+    """A kernel whose wait nothing ends gives up after its limit.  Each thread's next check raises, once, whichever
+    thread asks first, and the operators work as before."""
+    from sigcomp_b200 import _lib
+
+    def check():
+        try:
+            ops.check_waits()
+        except _lib.CodecError as e:
+            return "timed out" in str(e)
+        return False
+
+    ask, answers = threading.Barrier(2, timeout=60), []
+
+    def other():
+        torch.cuda.set_device(0)
+        check()                          # what was before
+        ask.wait()
+        ask.wait()
+        answers.append(check())
+        answers.append(check())
+
+    thread = threading.Thread(target=other)
+    thread.start()
+    check()
+    ask.wait()
+    _lib.check(_lib.load().sc_selftest_int8_wait_timeout(0, torch.cuda.current_stream().cuda_stream))
+    assert check() and not check()
+    ask.wait()
+    thread.join()
+    assert answers == [True, False]
+    x, (w, ws, b) = torch.randn(3000, 512, device=DEV), layer(512, 512, 1)
+    q, s = want_quantized(host(x))
+    same(ops.int8_linear(x, w, ws, b), want_linear(q, s, host(w), host(ws), host(b), False))
+    assert not check()
