@@ -72,6 +72,7 @@ struct DeviceGuard {
 int map_cuda(const CudaError &e)
 {
     set_error("CUDA error %s (%s) in %s", cudaGetErrorName(e.code), cudaGetErrorString(e.code), e.where.c_str());
+    cudaGetLastError();                  // the status reports it; the caller's own CUDA calls are not to find it
     return e.code == cudaErrorMemoryAllocation ? SC_ERR_OUT_OF_MEMORY : SC_ERR_CUDA;
 }
 

@@ -178,3 +178,23 @@ def test_a_wait_that_gives_up_is_reported_to_every_thread(ops):
     q, s = want_quantized(host(x))
     same(ops.int8_linear(x, w, ws, b), want_linear(q, s, host(w), host(ws), host(b), False))
     assert not check()
+
+
+# ---- errors of the CUDA runtime ----------------------------------------------------------------
+
+def test_a_failed_call_leaves_no_error_behind(ops):
+    """The runtime keeps a failed call's error for the thread until someone asks for it.  Torch asks after each of its
+    launches, so an error that is returned as a status must not be left for it."""
+    import ctypes
+    from sigcomp_b200 import _lib
+    L = _lib.load()
+    runtime = next(line.split()[-1] for line in open("/proc/self/maps") if "libcudart" in line)
+    last = ctypes.CDLL(runtime).cudaGetLastError
+    last()
+    some = 4096                                                # not read: there is no device 9999
+    assert L.sc_quantize_tokens_device(9999, some, 0, 4, 8, 8, some, 8, some, None) == _lib.SC_ERR_CUDA
+    assert last() == 0
+    assert L.sc_int8_status_device(9999, None) == _lib.SC_ERR_CUDA
+    assert last() == 0
+    x = torch.ones(8, device=DEV)
+    assert torch.cuda.current_device() == 0 and (x + 1).sum().item() == 16
