@@ -49,3 +49,17 @@ def test_tangents_are_refused(name):
 def test_derivatives_by_function_transforms_are_refused(transform):
     with pytest.raises((ValueError, RuntimeError), match="derivative|gradient|storage"):
         transform(lambda x: int8_linear(x, W, T).sum())
+
+
+# ---- build -------------------------------------------------------------------------------------
+
+def test_build_refuses_spills_in_the_kernels_that_load_tensor_memory():
+    """Both int8 kernels read TMEM into registers asynchronously: neither may spill."""
+    import re
+    from sigcomp_b200 import build_ext
+    loading = set()
+    for name in ("sc_int8.cu", "sc_int8_mm.cuh", "sc_int8_token.cuh"):
+        parts = re.split(r"__global__", (build_ext.CSRC / name).read_text())[1:]
+        loading |= {re.search(r"\b(k_\w+)\(", p).group(1) for p in parts if "tmem_ld" in p}
+    assert loading == {"k_pair", "k_few"}
+    assert loading <= set(build_ext.NO_SPILL_KERNELS) and "sc_int8.cu" in build_ext.NO_SPILL_SOURCES
