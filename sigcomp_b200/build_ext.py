@@ -11,6 +11,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libsigcomp_b200.so"
 BINDING = PKG / "_int8.so"
 BINDING_SOURCE = CSRC / "sc_torch.cpp"
+BINDING_STAMP = PKG / "_build" / "_int8.built_for"
 SOURCES = ["sc_capi.cu", "sc_codec.cu", "sc_frames.cu", "sc_int8.cu", "sc_mlp_simple.cu", "sc_mlp_tc.cu", "sc_signal.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
@@ -53,11 +54,22 @@ def _stale():
     return any(d.stat().st_mtime > t for d in deps if d.exists())
 
 
+def _built_for():
+    """What the binding is compiled against, beside its own sources."""
+    import torch
+    return f"torch {torch.__version__}, python {sys.version_info.major}.{sys.version_info.minor}"
+
+
+def _binding_stale():
+    if not BINDING.exists() or not BINDING_STAMP.exists() or BINDING_STAMP.read_text() != _built_for():
+        return True
+    header = PKG.parent / "include" / "sigcomp_b200.h"
+    return BINDING.stat().st_mtime <= max(f.stat().st_mtime for f in (BINDING_SOURCE, header, Path(__file__)))
+
+
 def build_binding(force=False, verbose=False):
     """The torch binding of the int8 operators, linked against libsigcomp_b200.so beside it."""
-    header = PKG.parent / "include" / "sigcomp_b200.h"
-    if not force and BINDING.exists() and BINDING.stat().st_mtime > max(
-            f.stat().st_mtime for f in (BINDING_SOURCE, header, Path(__file__))):
+    if not force and not _binding_stale():
         return BINDING
     import torch
     from torch.utils.cpp_extension import include_paths
@@ -65,6 +77,7 @@ def build_binding(force=False, verbose=False):
     tmp = BINDING.with_suffix(".so.tmp")
     includes = [sysconfig.get_paths()["include"], *include_paths(), "/usr/local/cuda/include"]
     cmd = ["/usr/bin/g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f'-DSC_TORCH_VERSION="{torch.__version__}"',
            *(a for d in includes for a in ("-isystem", str(d))), str(BINDING_SOURCE), "-o", str(tmp), f"-L{PKG}",
            f"-l:{LIB.name}", f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
            "-Wl,-rpath,$ORIGIN"]
@@ -72,6 +85,8 @@ def build_binding(force=False, verbose=False):
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)
     os.replace(tmp, BINDING)
+    BINDING_STAMP.parent.mkdir(exist_ok=True)
+    BINDING_STAMP.write_text(_built_for())
     return BINDING
 
 

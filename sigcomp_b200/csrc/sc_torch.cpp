@@ -350,4 +350,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "sigcomp_b200._int8", nullptr, -1, 
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject *PyInit__int8(void) { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject *PyInit__int8(void)
+{
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", SC_TORCH_VERSION) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

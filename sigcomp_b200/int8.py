@@ -32,6 +32,9 @@ try:
 except ImportError as exc:
     raise ImportError("sigcomp_b200/_int8.so is missing or does not load: build it with "
                       "`python -m sigcomp_b200.build_ext`") from exc
+if _int8.torch_version != torch.__version__:
+    raise ImportError(f"sigcomp_b200/_int8.so was built for torch {_int8.torch_version}, not {torch.__version__}: "
+                      "build it with `python -m sigcomp_b200.build_ext`")
 
 MAX_K = 131071
 

@@ -63,3 +63,21 @@ def test_build_refuses_spills_in_the_kernels_that_load_tensor_memory():
         loading |= {re.search(r"\b(k_\w+)\(", p).group(1) for p in parts if "tmem_ld" in p}
     assert loading == {"k_pair", "k_few"}
     assert loading <= set(build_ext.NO_SPILL_KERNELS) and "sc_int8.cu" in build_ext.NO_SPILL_SOURCES
+
+
+def test_binding_of_another_torch_is_rebuilt_and_not_used(monkeypatch, tmp_path):
+    """The binding is compiled against torch's headers: another version of torch makes it stale."""
+    import subprocess
+    import sys
+    from sigcomp_b200 import build_ext
+    done = subprocess.run([sys.executable, "-c", "import torch; torch.__version__ = '9.9.0'; import sigcomp_b200.int8"],
+                          cwd=build_ext.PKG.parent, capture_output=True, text=True)
+    assert done.returncode != 0 and "was built for torch" in done.stderr
+    monkeypatch.setattr(build_ext, "BINDING", tmp_path / "_int8.so")
+    monkeypatch.setattr(build_ext, "BINDING_STAMP", tmp_path / "stamp")
+    build_ext.BINDING.write_bytes(b"")
+    assert build_ext._binding_stale()                      # built for an unknown torch
+    build_ext.BINDING_STAMP.write_text(build_ext._built_for())
+    assert not build_ext._binding_stale()
+    monkeypatch.setattr(torch, "__version__", "9.9.0")
+    assert build_ext._binding_stale()
