@@ -397,45 +397,6 @@ __device__ __forceinline__ float affine(int32_t acc, float s, float t, float b, 
     return relu ? max_nan(y, 0.0f) : y;
 }
 
-// Any sizes, strides and alignment: 64 x 64 results a block, K in blocks of 64, CUDA cores.
-template <typename T>
-__global__ void __launch_bounds__(256)
-k_product_any(const int8_t *__restrict__ x, int64_t x_stride, const float *__restrict__ xs, const int8_t *__restrict__ w,
-              int64_t w_stride, const float *__restrict__ ws, const float *__restrict__ bias, int64_t rows, int n, int k,
-              int relu, T *__restrict__ y, int64_t y_stride)
-{
-    __shared__ int32_t a[64][17], b[64][17];
-    const int64_t m0 = (int64_t)blockIdx.x * 64;
-    const int n0 = blockIdx.y * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    int32_t acc[4][4] = {};
-    for (int k0 = 0; k0 < k; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-            const int r = i >> 6, c = i & 63;
-            const bool in = k0 + c < k;
-            reinterpret_cast<int8_t *>(a[r])[c] = in && m0 + r < rows ? x[(m0 + r) * x_stride + k0 + c] : 0;
-            reinterpret_cast<int8_t *>(b[r])[c] = in && n0 + r < n ? w[(int64_t)(n0 + r) * w_stride + k0 + c] : 0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[ty + 16 * i][c], b[tx + 16 * j][c], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = m0 + ty + 16 * i;
-            const int c = n0 + tx + 16 * j;
-            if (r < rows && c < n)
-                y[r * y_stride + c] = from_f32<T>(affine(acc[i][j], xs[r], ws[c], bias ? bias[c] : 0.0f, relu));
-        }
-}
-
 // sat(rint(y / scale)) in the low byte; a NaN becomes 0
 __device__ __forceinline__ uint32_t static_bits(float y, float scale)
 {

@@ -20,7 +20,7 @@ struct TokenParams {
     const int8_t *w;
     int64_t w_stride;
     const float *ws, *bias;
-    int64_t rows;
+    int64_t rows;                    // the kernel's MT
     int n, k, relu, y_type;
     void *y;
     int64_t y_stride;
@@ -64,7 +64,6 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
     uint32_t *tops = reinterpret_cast<uint32_t *>(red + (p.per_cta << p.log_s) * MT);   // [warps]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c0 = blockIdx.x * p.per_cta;
-    const int64_t t0 = (int64_t)blockIdx.y * MT;
 
     // this warp's channel group and part of K; steps of 32 vectors
     const int slot = warp >> p.log_s, seg = warp & (S - 1);
@@ -100,27 +99,22 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
         const bool packed = ((uintptr_t)x & 15) == 0 && (p.x_stride & 15) == 0;
 #pragma unroll 1
         for (int t = 0; t < MT; ++t) {
-            const int8_t *row = x + (t0 + t) * p.x_stride;
-            const bool live = t0 + t < p.rows;
+            const int8_t *row = x + (int64_t)t * p.x_stride;
             for (int v = threadIdx.x; v < kv; v += TK_THREADS)
                 *reinterpret_cast<uint4 *>(xq + t * kpad + v * 16) =
-                    !live ? make_uint4(0, 0, 0, 0)
-                          : packed && v * 16 + 16 <= p.k ? *reinterpret_cast<const uint4 *>(row + v * 16)
-                                                         : last_vec(row, v * 16, p.k);
+                    packed && v * 16 + 16 <= p.k ? *reinterpret_cast<const uint4 *>(row + v * 16) : last_vec(row, v * 16, p.k);
         }
-        if (threadIdx.x < MT) xs[threadIdx.x] = t0 + threadIdx.x < p.rows ? p.xs[t0 + threadIdx.x] : 0.0f;
+        if (threadIdx.x < MT) xs[threadIdx.x] = p.xs[threadIdx.x];
     } else {
         using V = Vec<typename std::conditional<sizeof(X) == 1, float, X>::type>;
         using E = typename std::conditional<sizeof(X) == 1, float, X>::type;
         constexpr int PER = TK_WARPS / MT;                                 // warps of a token
         const int t = warp / PER, th = (warp % PER) * 32 + lane;
-        const E *row = reinterpret_cast<const E *>(p.x) + (t0 + t) * p.x_stride;
-        const bool live = t0 + t < p.rows;
+        const E *row = reinterpret_cast<const E *>(p.x) + (int64_t)t * p.x_stride;
         const bool packed = ((uintptr_t)p.x & 15) == 0 && (p.x_stride * sizeof(E) & 15) == 0;
         uint32_t m = 0;
-        if (live)
-            for (int c = th * V::N; c < p.k; c += PER * 32 * V::N)
-                m = V::top(packed && c + V::N <= p.k ? *reinterpret_cast<const uint4 *>(row + c) : load_elements<E>(row + c, row, row + p.k), m);
+        for (int c = th * V::N; c < p.k; c += PER * 32 * V::N)
+            m = V::top(packed && c + V::N <= p.k ? *reinterpret_cast<const uint4 *>(row + c) : load_elements<E>(row + c, row, row + p.k), m);
         m = __reduce_max_sync(0xffffffffu, V::top_bits(m));
         if (lane == 0) tops[warp] = m;
         __syncthreads();
@@ -130,7 +124,7 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
         if (th == 0) xs[t] = rs.finite ? rs.s : __uint_as_float(0x7fc00000u);
         for (int c = th * V::N; c < kpad; c += PER * 32 * V::N) {
             uint32_t o[V::N / 4] = {};
-            if (live && rs.finite && c < p.k)
+            if (rs.finite && c < p.k)
                 V::quantise(packed && c + V::N <= p.k ? *reinterpret_cast<const uint4 *>(row + c) : load_elements<E>(row + c, row, row + p.k), rs.r, o);
 #pragma unroll
             for (int i = 0; i < V::N / 4; ++i) *reinterpret_cast<uint32_t *>(xq + t * kpad + c + 4 * i) = o[i];
@@ -181,12 +175,12 @@ __global__ void __launch_bounds__(TK_THREADS, 2) k_token(const TokenParams p)
     // the results, neighbouring threads on neighbouring channels
     for (int i = threadIdx.x; i < MT * p.per_cta; i += TK_THREADS) {
         const int t = i / p.per_cta, ch = i % p.per_cta, c = c0 + ch;
-        if (c >= p.n || t0 + t >= p.rows) continue;
+        if (c >= p.n) continue;
         int32_t sum = 0;
         for (int g = 0; g < S; ++g) sum += red[((ch << p.log_s) + g) * MT + t];
         const bool is_first = i == (int)threadIdx.x;
         const float y = affine(sum, xs[t], is_first ? ws0 : p.ws[c], is_first ? bias0 : p.bias ? p.bias[c] : 0.0f, p.relu);
-        store_one(p.y, p.y_type, (t0 + t) * p.y_stride + c, y, p.output_scale);
+        store_one(p.y, p.y_type, (int64_t)t * p.y_stride + c, y, p.output_scale);
     }
 }
 
