@@ -341,6 +341,18 @@ SC_API int sc_int8_linear_device(int device, const void *x, int32_t x_type, int6
 SC_API int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_packed, int64_t rows, int64_t n,
                                         int64_t k, int32_t y_type, int32_t y_scaled);
 
+/* How a call with these sizes is computed (host only; instrumentation): the number of parts that its rows
+ * are cut into, 1 or 2, and for each part five numbers in ways[10]: rows, kernel (SC_INT8_*), tokens of a
+ * tile of k_few (else 0), CTAs that split K, and the nanoseconds that the part is expected to take.  0 for
+ * sizes that the call refuses. */
+#define SC_INT8_TOKEN       0    /* one or two rows on CUDA cores */
+#define SC_INT8_FEW         1    /* k_few */
+#define SC_INT8_FEW_ROWS    2    /* k_few, rows quantised in the same launch */
+#define SC_INT8_PAIRS       3    /* k_pair */
+#define SC_INT8_PAIRS_ROWS  4    /* k_pair, rows quantised in the same launch */
+#define SC_INT8_PAIRS_TWICE 5    /* k_pair twice: the rows' maxima, then the rows */
+SC_API int sc_int8_linear_ways(int64_t rows, int64_t n, int64_t k, int32_t y_scaled, int64_t *ways);
+
 /* Waits for `stream` and reports whether a device-side wait of an int8 operator has timed out on
  * the device since the calling host thread's last such report, or, in its first, since the library
  * was loaded (SC_ERR_CUDA, as the other entry points report it; the results of the calls since then

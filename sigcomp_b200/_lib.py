@@ -27,6 +27,7 @@ EXPORTS = (
     "sc_decode_logits_device", "sc_frame_reads", "sc_unframe_reads", "sc_linear_layer_device",
     "sc_quantize_tokens_device", "sc_dequantize_tokens_device", "sc_int8_linear_device",
     "sc_int8_linear_workspace", "sc_int8_status_device", "sc_selftest_int8_wait_timeout",
+    "sc_int8_linear_ways",
 )
 
 KERNEL_KINDS = ("windows", "layer0", "hidden", "last_layer", "cdf_select", "encode", "compact", "decode_step",
@@ -71,6 +72,7 @@ def load():
     L.sc_int8_linear_device.argtypes = [ctypes.c_int, vp, i32, i64, vp, vp, i64, vp, vp, i64, i64, i64, i32, vp, i32,
                                         i64, vp, f32, vp, i64, vp]
     L.sc_int8_linear_workspace.argtypes = [i32, i32, i32, i64, i64, i64, i32, i32]
+    L.sc_int8_linear_ways.argtypes = [i64, i64, i64, i32, vp]
     L.sc_int8_status_device.argtypes = [ctypes.c_int, vp]
     L.sc_selftest_int8_wait_timeout.argtypes = [ctypes.c_int, vp]
     L.sc_int8_linear_workspace.restype = i64
@@ -89,7 +91,7 @@ def load():
                  "sc_selftest_wait_timeout", "sc_encode_logits_device", "sc_decode_logits_device",
                  "sc_frame_reads", "sc_unframe_reads", "sc_linear_layer_device",
                  "sc_quantize_tokens_device", "sc_dequantize_tokens_device", "sc_int8_linear_device",
-                 "sc_int8_status_device", "sc_selftest_int8_wait_timeout"):
+                 "sc_int8_status_device", "sc_selftest_int8_wait_timeout", "sc_int8_linear_ways"):
         getattr(L, name).restype = ctypes.c_int
     _lib = L
     return L

@@ -828,6 +828,12 @@ int64_t sc_int8_linear_workspace(int32_t x_type, int32_t x_packed, int32_t w_pac
     return int8_linear_workspace(p);
 }
 
+int sc_int8_linear_ways(int64_t rows, int64_t n, int64_t k, int32_t y_scaled, int64_t *ways)
+{
+    if (!ways || k > SC_INT8_MAX_K || !rows_ok(rows, n, n) || !rows_ok(n, k, k) || rows == 0) return 0;
+    return int8_linear_ways(rows, n, k, y_scaled != 0, ways);
+}
+
 int sc_int8_linear_device(int device, const void *x, int32_t x_type, int64_t x_stride, const float *x_scales,
                           const int8_t *w, int64_t w_stride, const float *w_scales, const float *bias, int64_t rows,
                           int64_t n, int64_t k, int32_t relu, void *y, int32_t y_type, int64_t y_stride,

@@ -720,7 +720,8 @@ int cluster_room(int ctas)
 // What multiplies a number of rows: the kernel, its tile and split, whether the rows are quantised by a launch of
 // their own, and the time in microseconds that it is expected to take.
 struct Way {
-    enum { TOKEN, FEW, FEW_ROWS, PAIRS, PAIRS_ROWS, PAIRS_TWICE } kernel;
+    enum { TOKEN = SC_INT8_TOKEN, FEW = SC_INT8_FEW, FEW_ROWS = SC_INT8_FEW_ROWS, PAIRS = SC_INT8_PAIRS,
+           PAIRS_ROWS = SC_INT8_PAIRS_ROWS, PAIRS_TWICE = SC_INT8_PAIRS_TWICE } kernel;
     int bt, split;
     TokenPlan t;
     bool requant;
@@ -844,6 +845,19 @@ static Plan plan(const Int8Linear &p)
 }
 
 int64_t int8_linear_workspace(const Int8Linear &p) { return plan(p).bytes; }
+
+int int8_linear_ways(int64_t rows, int64_t n, int64_t k, bool rows_out, int64_t *out)
+{
+    const Ways o = cut_rows(rows, n, k, rows_out);
+    const int parts = o.cut < rows ? 2 : 1;
+    for (int i = 0; i < parts; ++i) {
+        const Way &w = o.way[i];
+        const int64_t values[5] = {i == 0 ? o.cut : rows - o.cut, w.kernel, w.kernel == Way::FEW ? w.bt : 0, w.split,
+                                   (int64_t)(w.time * 1e3)};
+        std::copy(values, values + 5, out + 5 * i);
+    }
+    return parts;
+}
 
 // p's rows, x and w being int8 rows that TMA can read (k_token: as they are); `wide` takes a product in 32 bits
 static void multiply(const Int8Linear &p, const Way &way, Rows8 x, const float *xs, Rows8 w, float *wide, cudaStream_t s)

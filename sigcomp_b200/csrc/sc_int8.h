@@ -33,6 +33,8 @@ void quantize_tokens(const void *x, int type, int64_t rows, int64_t cols, int64_
 void dequantize_tokens(const int8_t *q, int64_t q_stride, const float *scales, float scale, int64_t rows, int64_t cols,
                        void *y, int type, int64_t y_stride, cudaStream_t s);
 int64_t int8_linear_workspace(const Int8Linear &p);
+// the parts that a call's rows are computed in, see sc_int8_linear_ways
+int int8_linear_ways(int64_t rows, int64_t n, int64_t k, bool rows_out, int64_t *out);
 void int8_linear(const Int8Linear &p, cudaStream_t s);
 
 }  // namespace sc

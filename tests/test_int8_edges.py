@@ -81,3 +81,41 @@ def test_binding_of_another_torch_is_rebuilt_and_not_used(monkeypatch, tmp_path)
     assert not build_ext._binding_stale()
     monkeypatch.setattr(torch, "__version__", "9.9.0")
     assert build_ext._binding_stale()
+
+
+# ---- the ways of a call ------------------------------------------------------------------------
+
+def _ways(rows, k, n, scaled):
+    """((rows, kernel, tile, split, ns), ...) of a call's parts."""
+    import ctypes
+    from sigcomp_b200 import _lib
+    out = (ctypes.c_int64 * 10)()
+    parts = _lib.load().sc_int8_linear_ways(rows, n, k, scaled, out)
+    return tuple(tuple(out[5 * i:5 * i + 5]) for i in range(parts))
+
+
+def test_ways_hold_all_rows():
+    for scaled in (0, 1):
+        for shape in ((1, 1, 1), (20480, 8192, 512), (9473, 2048, 300), (2 ** 31 - 1025, 1, 1)):
+            ways = _ways(*shape, scaled)
+            assert sum(w[0] for w in ways) == shape[0] and all(w[0] > 0 and w[4] > 0 for w in ways)
+    for shape in ((0, 8, 8), (-1, 8, 8), (8, 0, 8), (8, 8, 0), (8, 131072, 8), (2 ** 31, 8, 8)):
+        assert _ways(*shape, 1) == ()
+
+
+def test_tested_shapes_reach_every_way():
+    """Kernels, tiles and cuts that the sizes of a wide grid choose are all reached by the shapes that the GPU tests compare
+    with the definition."""
+    import test_gpu_int8
+    import test_gpu_int8_ways
+    tested = test_gpu_int8.SIZES + test_gpu_int8_ways.WHOLE + test_gpu_int8_ways.CUT
+
+    def kinds(shapes):
+        return {(scaled,) + tuple(w[1:3] for w in _ways(*shape, scaled)) for shape in shapes for scaled in (0, 1)}
+
+    grid = [(rows, k, n) for rows in (1, 2, 3, 8, 20, 60, 200, 1000, 3000, 9473, 10000, 18945, 19000, 19200, 20480, 38000, 40000)
+            for k in (64, 512, 2048, 4096, 8192) for n in (8, 96, 256, 300, 512, 700, 1300, 2304, 4096)]
+    assert kinds(grid) - kinds(tested) == set()
+    # K of k_few's tiles split in every number of parts
+    splits = {w[2:4] for shape in tested for scaled in (0, 1) for w in _ways(*shape, scaled) if w[1] == 1}
+    assert splits >= {w[2:4] for shape in grid for scaled in (0, 1) for w in _ways(*shape, scaled) if w[1] == 1}
