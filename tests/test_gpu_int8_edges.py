@@ -198,3 +198,50 @@ def test_a_failed_call_leaves_no_error_behind(ops):
     assert last() == 0
     x = torch.ones(8, device=DEV)
     assert torch.cuda.current_device() == 0 and (x + 1).sum().item() == 16
+
+
+# ---- decoding ----------------------------------------------------------------------------------
+
+def test_decoding_step_by_step(ops):
+    """A model whose next logits depend on the symbols decoded before: each step computes one row of logits per stream,
+    from the decoded symbols alone, and decodes the streams' prefixes with the rows so far."""
+    import ctypes
+    from sigcomp_b200 import _lib
+    from sigcomp_b200.codec import B200Compression
+    from sigcomp_b200.model import random_model
+    model = random_model(3)
+    codec = B200Compression(chunk_len=2048, gpu=0, model=model)
+    streams, steps, window = 5, 24, model.window_size
+    table = torch.from_numpy(model.embedding.astype(np.float32)).to(torch.bfloat16).to(DEV)
+    layers = [layer(512, window * model.emb_dim, 1), layer(512, 512, 2), layer(256, 512, 3)]
+    scale = float(model.output_scale)
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+
+    def logits_of(ids):
+        q, s = ops.quantize_tokens(table[ids].flatten(-2))
+        for l in layers[:-1]:
+            q, s = ops.int8_linear_requant(q, s, *l, relu=True)
+        return ops.int8_linear_requant(q, s, *layers[-1], output_scale=scale)
+
+    symbols = np.random.default_rng(1).integers(0, 256, size=(streams, steps)).astype(np.uint8)
+    sym = torch.from_numpy(symbols).to(DEV)
+    known = torch.cat([torch.full((streams, window), 256, device=DEV), sym.long()], dim=1)
+    batch = logits_of(known.unfold(1, window, 1)[:, :steps]).contiguous()
+    off = torch.arange(0, streams * steps + 1, steps, dtype=torch.int64, device=DEV)
+    words = torch.zeros(streams * (steps + 2), dtype=torch.int32, device=DEV)
+    woff = torch.zeros(streams + 1, dtype=torch.int64, device=DEV)
+    _lib.check(codec._lib.sc_encode_logits_device(codec.handle, p(batch), p(sym.contiguous()), p(off), streams, p(words),
+                                                  words.numel(), p(woff), None, st))
+    context = torch.full((streams, window), 256, device=DEV)
+    rows, back = [], None
+    for t in range(steps):
+        rows.append(logits_of(context))
+        so_far = torch.stack(rows, dim=1).contiguous()
+        back = torch.zeros((streams, t + 1), dtype=torch.uint8, device=DEV)
+        off = torch.arange(0, streams * (t + 1) + 1, t + 1, dtype=torch.int64, device=DEV)
+        _lib.check(codec._lib.sc_decode_logits_device(codec.handle, p(so_far), p(off), p(words), p(woff), streams, p(back),
+                                                      None, st))
+        context = torch.cat([context[:, 1:], back[:, t:].long()], dim=1)
+    assert torch.equal(back, sym)
+    codec.close()
