@@ -178,6 +178,8 @@ SC_API int sc_encode_logits_device(sc_model *model, const int8_t *logits, const 
  * decode_step_int8 at every step; semantics of CpuRangeDecoder and _decode_partition,
  * cpu_entropy_coding.py:230-266, 451-481).  Device memory; stream_errors as in
  * sc_decompress_chunks (SC_ERR_CORRUPT_STREAM names the first invalid stream).
+ * Each call decodes its streams from their first symbol on: no state is kept between calls.
+ * Fewer rows than were coded give a stream's first symbols.
  */
 SC_API int sc_decode_logits_device(sc_model *model, const int8_t *logits, const int64_t *offsets,
                                    const uint32_t *words, const int64_t *word_offsets, int64_t n_streams,

@@ -729,8 +729,9 @@ struct Way {
 };
 
 // The way that is expected to take least.  The times are so many waves of CTAs, each of them a start and an end plus
-// its K blocks, and about 2 us for a launch that quantises rows; fitted to measurements at 1 to 20,480 rows of
-// seven layers (512 x 512 to 8,192 x 2,048).  Among them, k_few against k_pair:
+// its K blocks, and about 2 us for a launch that quantises rows; fitted to measurements.  At 1 to 20,480 rows of
+// seven layers (512 x 256 to 4,096 x 4,096) calls take 0.74 to 1.40 times what is expected, 1.02 in the median.  Among
+// them, k_few against k_pair:
 //   K = 512, N = 512:     16 rows 3.4 / 5.9,  1,000 rows 4.5 / 6.5,  3,000 rows 7.9 / 6.2
 //   K = 8,192, N = 512:   16 rows 5.2 / 22,  1,000 rows 12.1 / 23,  3,000 rows 24.1 / 22.8
 //   K = 4,096, N = 4,096: 16 rows 6.0 / 13.8,  400 rows 15.8 / 14.4,  1,000 rows 29.9 / 15.3
@@ -764,8 +765,8 @@ Way choose(int64_t rows, int64_t n, int64_t k, bool rows_out)
                 offer(Way::FEW_ROWS, 16, split, false, 3.2 + 0.24 * (double)((nkb + split - 1) / split));
         if (blocks <= 2)
             offer(Way::PAIRS_ROWS, 0, 1, false, 4.2 + waves(tiles, pairs) * ((double)blocks * 0.3 * (double)nkb + 2.9));
-        // both launches multiply; nothing in 32 bits leaves the chip (28,467 rows of 128 x 4,650: 156 us against 292,
-        // 20,480 of 1,024 x 1,024: 42 against 54)
+        // both launches multiply; nothing in 32 bits leaves the chip (28,467 rows of 128 x 4,650: 181 us against 282,
+        // 20,480 of 1,024 x 1,024: 43 against 46)
         offer(Way::PAIRS_TWICE, 0, 1, false,
               10.0 + waves(tiles * blocks, pairs) * (2 * std::max(0.3 * (double)nkb, 0.2) + 2.6));
     }

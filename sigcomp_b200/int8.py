@@ -12,8 +12,9 @@ and whose activations are quantised token by token as they come, is computed wit
 
 A row's result depends neither on the rows beside it nor on their number: sums of products are
 whole numbers, exact in 32 bits, and the roundings after them are fixed (include/sigcomp_b200.h
-writes them out).  So teacher-forced coding in large batches and decoding token by token agree bit
-for bit.
+writes them out).  So logits computed in large batches for coding and row by row for decoding agree
+bit for bit.  (``sc_decode_logits_device`` starts every stream anew, so a decoder whose next logits
+depend on the last symbol passes the rows of all steps so far.)
 
 Arrays are torch tensors on one GPU; leading dimensions are batch dimensions.  Rows of every result
 start a multiple of 16 bytes apart, so results are contiguous where their width is such a multiple, and
