@@ -66,11 +66,13 @@ const at::Tensor &tensor(const char *name, PyObject *o, int types, const at::Ten
     if (t.layout() != c10::kStrided || t.is_neg()) refuse("%s must be a dense tensor, not a lazily negated one", name);
     if (beside && t.device() != beside->device())
         refuse("%s is on %s, the other arrays are on %s", name, t.device().str().c_str(), beside->device().str().c_str());
-    if (t.requires_grad() && c10::GradMode::is_enabled())
-        refuse("%s asks for a gradient, which the int8 operators do not have", name);
-    // a dual tensor: its tangent would be lost
-    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
-        refuse("%s asks for a forward derivative, which the int8 operators do not have", name);
+    if (t.unsafeGetTensorImpl()->autograd_meta()) {                // without it a tensor has neither
+        if (t.requires_grad() && c10::GradMode::is_enabled())
+            refuse("%s asks for a gradient, which the int8 operators do not have", name);
+        // a dual tensor: its tangent would be lost
+        if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+            refuse("%s asks for a forward derivative, which the int8 operators do not have", name);
+    }
     return t;
 }
 
