@@ -245,3 +245,16 @@ def test_decoding_step_by_step(ops):
         context = torch.cat([context[:, 1:], back[:, t:].long()], dim=1)
     assert torch.equal(back, sym)
     codec.close()
+
+
+def test_a_result_that_does_not_fit_is_a_memory_error(ops):
+    """The allocation fails while Python's lock is released: the error is raised all the same, and calls work after it."""
+    rows = 2_000_000_000
+    q, s = torch.ones((1, 16), dtype=torch.int8, device=DEV), torch.ones(1, device=DEV)
+    w, ws, b = layer(64, 16, 1)
+    want = ops.int8_linear(q, w, ws, b, x_scales=s)
+    with pytest.raises(MemoryError):
+        ops.int8_linear(q.expand(rows, 16), w, ws, b, x_scales=s.expand(rows))             # 512 GB
+    with pytest.raises(MemoryError):
+        ops.dequantize_tokens(q.expand(3 * rows, 16), 1.0)
+    assert torch.equal(ops.int8_linear(q, w, ws, b, x_scales=s), want)
